@@ -9,5 +9,5 @@ B200 the calls raise.
 from . import _lib  # noqa: F401
 from .errors import CudaError, DeersError, DeviceMismatch, DTypeMismatch, LayoutMismatch  # noqa: F401
 
-__all__ = ["_lib", "ops", "shard", "DeersError", "CudaError", "DeviceMismatch", "DTypeMismatch",
+__all__ = ["_lib", "ops", "q8", "shard", "DeersError", "CudaError", "DeviceMismatch", "DTypeMismatch",
            "LayoutMismatch"]

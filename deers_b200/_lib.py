@@ -10,7 +10,8 @@ _HERE = os.path.dirname(os.path.abspath(__file__))
 LIB_PATH = os.path.join(_HERE, "lib", "libdeers_b200.so")
 
 OK, ERR_NULL, ERR_SHAPE, ERR_DTYPE, ERR_LAYOUT, ERR_WORKSPACE, ERR_CUDA, ERR_KERNEL, ERR_UNSUPPORTED, ERR_DEVICE = range(10)
-F16, F32 = 0, 1
+F16, F32, I8, E4M3 = range(4)
+CACHE_BLOCK = 32
 
 # Every symbol include/deers_b200.h declares.
 SYMBOLS = [
@@ -33,6 +34,8 @@ SYMBOLS = [
     "deers_b200_gpt_forward_backward", "deers_b200_gpt_train_step", "deers_b200_gpt_train_step_host",
     "deers_b200_shard_range", "deers_b200_comm_init_all", "deers_b200_comm_export", "deers_b200_comm_init_ipc",
     "deers_b200_comm_destroy", "deers_b200_comm_set_lanes", "deers_b200_allgather_o", "deers_b200_allgather_join", "deers_b200_allgather_flush",
+    "deers_b200_quantize_rows", "deers_b200_gemm_q8", "deers_b200_cache_q8_append", "deers_b200_attn_decode_q8_workspace_bytes",
+    "deers_b200_attn_decode_q8",
     "deers_b200_selftest_wait", "deers_b200_product_route", "deers_b200_split_f16x3", "deers_b200_gemm_f16x3_workspace_bytes", "deers_b200_gemm_f16x3",
 ]
 IPC_HANDLE_BYTES = 72
@@ -71,6 +74,23 @@ class DecodeDesc(ctypes.Structure):
                 ("D", ctypes.c_int32), ("dtype", ctypes.c_int32), ("causal", ctypes.c_int32), ("scale", ctypes.c_float),
                 ("q_strides", ctypes.c_int64 * 4), ("k_strides", ctypes.c_int64 * 4),
                 ("v_strides", ctypes.c_int64 * 4), ("o_strides", ctypes.c_int64 * 4)]
+
+
+class QuantizeDesc(ctypes.Structure):
+    _fields_ = [("rows", ctypes.c_int64), ("C", ctypes.c_int32), ("dtype", ctypes.c_int32), ("code", ctypes.c_int32), ("norm", ctypes.c_int32),
+                ("relu_squared", ctypes.c_int32), ("eps", ctypes.c_double)] + [(f"ld_{n}", ctypes.c_int64) for n in ("x", "residual", "sum", "codes")]
+
+
+class CacheQ8(ctypes.Structure):
+    _fields_ = [("B", ctypes.c_int32), ("H", ctypes.c_int32), ("capacity", ctypes.c_int32), ("D", ctypes.c_int32),
+                ("k", ctypes.c_void_p), ("v", ctypes.c_void_p), ("k_scale", ctypes.c_void_p), ("v_scale", ctypes.c_void_p),
+                ("k_strides", ctypes.c_int64 * 3), ("v_strides", ctypes.c_int64 * 3),
+                ("k_scale_strides", ctypes.c_int64 * 2), ("v_scale_strides", ctypes.c_int64 * 2)]
+
+
+class DecodeQ8Desc(ctypes.Structure):
+    _fields_ = [("cache", CacheQ8), ("H", ctypes.c_int32), ("Tq", ctypes.c_int32), ("dtype", ctypes.c_int32), ("causal", ctypes.c_int32),
+                ("scale", ctypes.c_float), ("q_strides", ctypes.c_int64 * 4), ("o_strides", ctypes.c_int64 * 4)]
 
 
 class GemmEpilogue(ctypes.Structure):
@@ -155,6 +175,13 @@ def lib() -> ctypes.CDLL:
     L.deers_b200_cross_entropy_scratch_bytes.restype = sz
     L.deers_b200_cross_entropy_fwd.argtypes = [vp, i64, i64, vp, i64, vp, vp, vp, vp, sz]
     L.deers_b200_cross_entropy_bwd.argtypes = [vp, i64, i64, vp, i64, vp, vp, ctypes.c_float, vp, i64]
+    L.deers_b200_quantize_rows.argtypes = [vp, ctypes.POINTER(QuantizeDesc), vp, vp, vp, vp, vp]
+    L.deers_b200_gemm_q8.argtypes = [vp, i32, i32, i32, i32, vp, i64, vp, vp, i64, vp, i32, vp, i64]
+    p64 = ctypes.POINTER(i64)
+    L.deers_b200_cache_q8_append.argtypes = [vp, ctypes.POINTER(CacheQ8), i32, i32, vp, p64, vp, p64, vp, vp]
+    L.deers_b200_attn_decode_q8_workspace_bytes.argtypes = [ctypes.POINTER(DecodeQ8Desc)]
+    L.deers_b200_attn_decode_q8_workspace_bytes.restype = sz
+    L.deers_b200_attn_decode_q8.argtypes = [vp, ctypes.POINTER(DecodeQ8Desc), vp, vp, vp, vp, vp, sz]
     gcp, hp = ctypes.POINTER(GptConfig), ctypes.POINTER(AdamWHyper)
     L.deers_b200_gpt_create.argtypes = [vp, gcp, ctypes.c_int32, ctypes.POINTER(vp)]
     L.deers_b200_gpt_destroy.argtypes = [vp]

@@ -1,0 +1,193 @@
+// New keys and values into a cache of e4m3 codes with a scale for every 32 tokens of a head.
+//
+// Row start[b] + t of sequence b receives new row t, t < count[b].  Of a block of 32 tokens that gets rows,
+//     scale' = max(scale if the block holds earlier rows of the sequence, max|new rows| * (1 / 448 in f32))
+// new codes are nearest(value / scale'), and where the scale has grown the block's earlier rows are rounded again, nearest(code * scale / scale');
+// other rows and blocks stay as they are.  So one scale serves a block however its rows arrive, a block that starts anew forgets what lay
+// there, and writing the same rows again changes nothing.  A value that is no number is stored as NaN and takes no part in the scale.
+// A group of threads (a warp, or four) owns a block of one head of keys or values: it reads the new rows once, into registers.
+// Bound: HBM, 3 bytes an element with f16; for single tokens the launch.
+#include "common.cuh"
+#include "q8_codes.cuh"
+
+namespace {
+
+struct AppendParams {
+    const void* src[2];                       // keys, values [B,H,T,D]
+    uint8_t* codes[2];                        // [B,H,cap,D]
+    float* scale[2];                          // [B,H,blocks]
+    long long ss[2][3], sc[2][3], sl[2][2];   // strides (b, h, t) in elements, of the scales (b, h)
+    const int* start; const int* count;       // count may be nullptr: T rows of every sequence
+    int H, T, D, cap;
+    unsigned int* err;
+};
+
+__device__ __forceinline__ float as_f(__half v) { return __half2float(v); }
+__device__ __forceinline__ float as_f(float v) { return v; }
+
+// 32 * NW threads own a token block; NP pieces of four values each stay in registers.
+template <typename T, bool VEC, int NW, int NP>
+__global__ void __launch_bounds__(128) append_q8_kernel(const AppendParams p) {
+    chain_begin();
+    constexpr int NT = 32 * NW, PER = 128 / NT;                  // groups of a block of threads
+    const int tid = threadIdx.x % NT, warp = threadIdx.x / 32;
+    const int h = blockIdx.y * PER + threadIdx.x / NT, b = blockIdx.z >> 1, kv = blockIdx.z & 1;
+    const bool mine = h < p.H;                                   // (with NW == 4 the whole block)
+    int begin = p.start[b], n = p.count ? p.count[b] : p.T;
+    if (begin < 0 || n < 0 || n > p.T || (long long)begin + n > p.cap) {      // rows outside of the cache are left out, and told
+        if (threadIdx.x == 0 && blockIdx.x == 0) atomicCAS(p.err, 0u, (unsigned)DEERS_KERR_CACHE | 1u);
+        n = min(max(n, 0), p.T);
+        if (begin < 0 || begin >= p.cap) n = 0;
+        n = min(n, p.cap - begin);
+    }
+    if (n <= 0 || !mine) return;
+    const int blk = begin / q8::BLOCK + blockIdx.x, first = blk * q8::BLOCK;
+    const int lo = max(begin, first), hi = min(begin + n, first + q8::BLOCK);
+    if (lo >= hi) return;
+    const T* src = static_cast<const T*>(p.src[kv]) + b * p.ss[kv][0] + h * p.ss[kv][1] + (long long)(lo - begin) * p.ss[kv][2];
+    uint8_t* codes = p.codes[kv] + b * p.sc[kv][0] + h * p.sc[kv][1];
+    float* scale_at = p.scale[kv] + b * p.sl[kv][0] + h * p.sl[kv][1] + blk;
+    const long long st = p.ss[kv][2], sc = p.sc[kv][2];
+    const int per_row = p.D / 4, pieces = (hi - lo) * per_row;
+    const float was = begin > first ? *scale_at : 0.f;
+    float v[NP][4];
+    unsigned top = 0;
+#pragma unroll
+    for (int i = 0; i < NP; ++i) {
+        const int at = tid + i * NT;
+        if (at < pieces) {
+            const T* s = src + at / per_row * st + at % per_row * 4;
+            if constexpr (VEC) {
+                T raw[4];
+                if constexpr (sizeof(T) == 2) *reinterpret_cast<uint2*>(raw) = *reinterpret_cast<const uint2*>(s);
+                else *reinterpret_cast<uint4*>(raw) = *reinterpret_cast<const uint4*>(s);
+#pragma unroll
+                for (int e = 0; e < 4; ++e) v[i][e] = as_f(raw[e]);
+            } else {
+#pragma unroll
+                for (int e = 0; e < 4; ++e) v[i][e] = as_f(s[e]);
+            }
+        }
+    }
+#pragma unroll
+    for (int i = 0; i < NP; ++i) {
+        if (tid + i * NT < pieces) {
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+                const unsigned bits = __float_as_uint(v[i][e]) & 0x7fffffffu;
+                if (bits < 0x7f800000u) top = max(top, bits);
+                else v[i][e] = __uint_as_float(0x7fc00000u);
+            }
+        }
+    }
+#pragma unroll
+    for (int off = 16; off >= 1; off >>= 1) top = max(top, __shfl_xor_sync(0xffffffffu, top, off));
+    if constexpr (NW > 1) {
+        __shared__ unsigned s_top[4];
+        if ((threadIdx.x & 31) == 0) s_top[warp] = top;
+        __syncthreads();
+#pragma unroll
+        for (int w = 0; w < NW; ++w) top = max(top, s_top[w]);
+    } else {
+        __syncwarp();                                            // every lane has read the old scale
+    }
+    const float fresh = __uint_as_float(top) * (1.0f / q8::MOST_E4M3);
+    const bool grown = fresh > was;
+    const float scale = grown ? fresh : was;
+    const float inf = __uint_as_float(0x7f800000u);
+    if (tid == 0) *scale_at = scale;
+    if (grown && begin > first) {                                // the earlier rows, 16 bytes at a time
+        const float again = was / scale;
+        const int per16 = p.D / 16, old16 = (begin - first) * per16;
+        for (int at = tid; at < old16; at += NT) {
+            uint4* c = reinterpret_cast<uint4*>(codes + (first + at / per16) * sc + at % per16 * 16);
+            const uint4 w = *c;
+            const uint32_t in[4] = {w.x, w.y, w.z, w.w};
+            uint32_t out[4];
+#pragma unroll
+            for (int k = 0; k < 4; ++k) {
+                float f[4];
+                q8::e4m3_values(in[k], f);
+                out[k] = q8::codes_of<false>(f, again, was, scale, false);
+            }
+            *c = make_uint4(out[0], out[1], out[2], out[3]);
+        }
+    }
+    const float r = scale > 0.f ? 1.0f / scale : 0.f;
+    const bool wide = !(r < inf);
+#pragma unroll
+    for (int i = 0; i < NP; ++i) {
+        const int at = tid + i * NT;
+        if (at < pieces) *reinterpret_cast<uint32_t*>(codes + (lo + at / per_row) * sc + at % per_row * 4) = q8::codes_of<false>(v[i], r, 1.0f, scale > 0.f ? scale : 1.0f, wide);
+    }
+}
+
+template <typename T, bool VEC>
+int append_launch(deers_ctx* ctx, const AppendParams& p, int B) {
+    // token blocks that T rows can touch from any place
+    const unsigned blocks = p.T < 2 ? 1u : (unsigned)((p.T - 2) / q8::BLOCK + 2);
+    const int rows = p.T < q8::BLOCK ? p.T : q8::BLOCK, pieces = rows * p.D / 4;         // of a token block, at most
+    KernelTimerScope ts(ctx, DEERS_K_DECODE);
+    const dim3 warps(blocks, (unsigned)((p.H + 3) / 4), 2u * B), whole(blocks, (unsigned)p.H, 2u * B);
+    if (pieces <= 64) DEERS_CUDA_TRY(ctx, launch_chained(ctx, append_q8_kernel<T, VEC, 1, 2>, warps, 128, 0, 1, p));
+    else if (pieces <= 256) DEERS_CUDA_TRY(ctx, launch_chained(ctx, append_q8_kernel<T, VEC, 1, 8>, warps, 128, 0, 1, p));
+    else if (pieces <= 1024) DEERS_CUDA_TRY(ctx, launch_chained(ctx, append_q8_kernel<T, VEC, 4, 8>, whole, 128, 0, 1, p));
+    else DEERS_CUDA_TRY(ctx, launch_chained(ctx, append_q8_kernel<T, VEC, 4, 16>, whole, 128, 0, 1, p));
+    return DEERS_OK;
+}
+
+}  // namespace
+
+int deers_check_cache(const deers_cache_q8* c) {
+    if (!c) return DEERS_ERR_NULL;
+    if (c->B < 1 || c->H < 1 || c->capacity < 1 || c->D < 1) return DEERS_ERR_SHAPE;
+    if (c->D % 16 || c->D > 256 || c->B > 32767 || c->H > 65535 || c->capacity > (1 << 24)) return DEERS_ERR_UNSUPPORTED;
+    if (!c->k || !c->v || !c->k_scale || !c->v_scale) return DEERS_ERR_NULL;
+    if (((uintptr_t)c->k | (uintptr_t)c->v) & 15u || ((uintptr_t)c->k_scale | (uintptr_t)c->v_scale) & 3u) return DEERS_ERR_LAYOUT;
+    for (int i = 0; i < 3; ++i)
+        if (c->k_strides[i] < 0 || c->v_strides[i] < 0 || (c->k_strides[i] | c->v_strides[i]) & 15) return DEERS_ERR_LAYOUT;
+    for (int i = 0; i < 2; ++i)
+        if (c->k_scale_strides[i] < 0 || c->v_scale_strides[i] < 0) return DEERS_ERR_LAYOUT;
+    if (c->k_strides[2] < c->D || c->v_strides[2] < c->D) return DEERS_ERR_LAYOUT;
+    return DEERS_OK;
+}
+
+extern "C" int deers_b200_cache_q8_append(deers_ctx* ctx, const deers_cache_q8* c, int32_t T, int32_t dtype, const void* k, const int64_t* k_strides,
+                                          const void* v, const int64_t* v_strides, const int32_t* start, const int32_t* count) {
+    if (!ctx || !c || !k_strides || !v_strides) return DEERS_ERR_NULL;
+    int rc = deers_check_cache(c);
+    if (rc) return rc;
+    if (dtype != DEERS_F16 && dtype != DEERS_F32) return DEERS_ERR_DTYPE;
+    if (T < 0 || T > c->capacity) return DEERS_ERR_SHAPE;
+    if (T == 0) return DEERS_OK;
+    if (!k || !v || !start) return DEERS_ERR_NULL;
+    const int64_t es = dtype == DEERS_F16 ? 2 : 4;
+    if (((uintptr_t)k | (uintptr_t)v) & (uintptr_t)(es - 1) || ((uintptr_t)start | (uintptr_t)count) & 3u) return DEERS_ERR_LAYOUT;
+    if (k_strides[3] != 1 || v_strides[3] != 1) return DEERS_ERR_LAYOUT;
+    const int64_t al = 4 * es;                                    // four values at a time
+    bool vec = (((uintptr_t)k | (uintptr_t)v) & (uintptr_t)(al - 1)) == 0;
+    AppendParams p;
+    for (int i = 0; i < 3; ++i) {
+        if (k_strides[i] < 0 || v_strides[i] < 0) return DEERS_ERR_LAYOUT;
+        // (a cache whose sequences or heads are one place can be read, not written)
+        if ((i == 0 ? c->B : i == 1 ? c->H : 1) > 1 && (c->k_strides[i] == 0 || c->v_strides[i] == 0)) return DEERS_ERR_LAYOUT;
+        vec = vec && ((k_strides[i] | v_strides[i]) & 3) == 0;
+        p.ss[0][i] = k_strides[i]; p.ss[1][i] = v_strides[i];
+        p.sc[0][i] = c->k_strides[i]; p.sc[1][i] = c->v_strides[i];
+    }
+    for (int i = 0; i < 2; ++i)
+        if ((i == 0 ? c->B : c->H) > 1 && (c->k_scale_strides[i] == 0 || c->v_scale_strides[i] == 0)) return DEERS_ERR_LAYOUT;
+    for (int i = 0; i < 2; ++i) { p.sl[0][i] = c->k_scale_strides[i]; p.sl[1][i] = c->v_scale_strides[i]; }
+    p.src[0] = k; p.src[1] = v;
+    p.codes[0] = (uint8_t*)c->k; p.codes[1] = (uint8_t*)c->v;
+    p.scale[0] = c->k_scale; p.scale[1] = c->v_scale;
+    p.start = start; p.count = count;
+    p.H = c->H; p.T = T; p.D = c->D; p.cap = c->capacity; p.err = ctx->dev_err;
+    DEERS_CUDA_TRY(ctx, cudaSetDevice(ctx->device));
+    const auto go = dtype == DEERS_F16 ? (vec ? append_launch<__half, true> : append_launch<__half, false>)
+                                       : (vec ? append_launch<float, true> : append_launch<float, false>);
+    if ((rc = go(ctx, p, c->B))) return rc;
+    ctx->launches += 1;
+    DEERS_CUDA_TRY(ctx, cudaGetLastError());
+    return DEERS_OK;
+}

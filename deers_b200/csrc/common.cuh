@@ -173,6 +173,7 @@ enum {
     DEERS_KERR_SELFTEST = 0x300,
     DEERS_KERR_GEMM = 0x400,
     DEERS_KERR_GPT = 0x500,      // token id / target out of range
+    DEERS_KERR_CACHE = 0x600,    // place or length outside of a cache
 };
 
 // Work schedule shared by the persistent f16 kernels (ctx.cu).  Work items are ordered in groups

@@ -15,6 +15,7 @@
 #include <ATen/cuda/CUDAContext.h>
 #include <ATen/cuda/EmptyTensor.h>
 #include <c10/cuda/CUDACachingAllocator.h>
+#include <c10/cuda/CUDAGuard.h>
 #include <c10/cuda/CUDAStream.h>
 #include <torch/csrc/autograd/python_variable.h>
 
@@ -372,6 +373,212 @@ PyObject* rope_pack(PyObject*, PyObject* const* args, Py_ssize_t n) {
     HOST_END
 }
 
+// ---- 8-bit operators (deers_b200/q8.py).  The device that was current stays so.
+inline int code_of(const at::Tensor& t) { return t.scalar_type() == at::kChar ? DEERS_I8 : t.scalar_type() == at::kFloat8_e4m3fn ? DEERS_E4M3 : -1; }
+inline bool on(const at::Tensor* t, int device) { return t && t->is_cuda() && t->get_device() == device; }
+// Rows of the last axis at one distance from one another, each contiguous.
+inline bool is_rows(const at::Tensor& t) { return t.is_contiguous() || (t.dim() == 2 && (t.stride(1) == 1 || t.size(1) == 1) && t.stride(0) >= 0); }
+inline int64_t row_stride(const at::Tensor& t) { return t.dim() == 2 ? t.stride(0) : t.size(-1); }
+
+// quantize_rows(x, residual | None, norm, relu_squared, eps, code) -> (sum | None, codes, scale) | None
+PyObject* quantize_rows(PyObject*, PyObject* const* args, Py_ssize_t n) {
+    HOST_BEGIN
+    if (n != 6) Py_RETURN_NONE;
+    const at::Tensor *x = tensor(args[0]), *res = args[1] == Py_None ? nullptr : tensor(args[1]);
+    if (!x || x->dim() < 1 || !x->is_cuda() || dtype_code(*x) < 0 || !is_rows(*x) || x->size(-1) < 1) Py_RETURN_NONE;
+    if (args[1] != Py_None && (!res || !same(*x, *res) || !res->is_cuda() || !is_rows(*res))) Py_RETURN_NONE;
+    deers_quantize_desc d;
+    memset(&d, 0, sizeof(d));
+    d.norm = PyObject_IsTrue(args[2]); d.relu_squared = PyObject_IsTrue(args[3]);
+    d.eps = PyFloat_AsDouble(args[4]);
+    if (d.eps == -1.0 && PyErr_Occurred()) return nullptr;
+    d.code = (int)PyLong_AsLong(args[5]);
+    if (d.code == -1 && PyErr_Occurred()) return nullptr;
+    const c10::cuda::CUDAGuard device(x->device());
+    Ctx* ctx = context_for(x->get_device());
+    if (!ctx) return nullptr;
+    const int64_t C = x->size(-1), ld = (C + 15) / 16 * 16;
+    if (C > 0x7fffffff - 16) Py_RETURN_NONE;
+    d.rows = x->numel() / C; d.C = (int)C; d.dtype = dtype_code(*x);
+    d.ld_x = row_stride(*x); d.ld_residual = res ? row_stride(*res) : 0; d.ld_sum = C; d.ld_codes = ld;
+    at::Tensor sum, codes, scale;
+    int rc;
+    {
+        NoGil unlocked;
+        const at::ScalarType st = d.code == DEERS_I8 ? at::kChar : at::kFloat8_e4m3fn;
+        if (res) sum = empty_like_of(x->sizes(), x->scalar_type(), *x);
+        if (ld == C) {
+            codes = empty_like_of(x->sizes(), st, *x);
+        } else {                                             // the padding is behind every row
+            codes = empty_like_of({d.rows, ld}, st, *x);
+            std::vector<int64_t> strides(x->dim(), 1);
+            int64_t step = ld;
+            for (int64_t i = x->dim() - 2; i >= 0; --i) { strides[i] = step; step *= x->size(i); }
+            codes = codes.as_strided(x->sizes(), strides);
+        }
+        scale = empty_like_of(x->sizes().slice(0, x->dim() - 1), at::kFloat, *x);
+        std::lock_guard<std::mutex> one(ctx->mu);
+        rc = deers_b200_quantize_rows(ctx->handle, &d, x->data_ptr(), res ? res->data_ptr() : nullptr, res ? sum.data_ptr() : nullptr, codes.data_ptr(),
+                                      (float*)scale.data_ptr());
+    }
+    if (rc) return fail(rc, ctx);
+    PyObject* r = PyTuple_New(3);
+    if (res) PyTuple_SET_ITEM(r, 0, THPVariable_Wrap(std::move(sum)));
+    else { Py_INCREF(Py_None); PyTuple_SET_ITEM(r, 0, Py_None); }
+    PyTuple_SET_ITEM(r, 1, THPVariable_Wrap(std::move(codes)));
+    PyTuple_SET_ITEM(r, 2, THPVariable_Wrap(std::move(scale)));
+    return r;
+    HOST_END
+}
+
+// gemm_q8(a, a_scale, b, b_scale, out_dtype) -> c | None.  a [.., K], b [N, K] codes with rows on 16-byte boundaries.
+PyObject* gemm_q8(PyObject*, PyObject* const* args, Py_ssize_t n) {
+    HOST_BEGIN
+    if (n != 5) Py_RETURN_NONE;
+    const at::Tensor *a = tensor(args[0]), *sa = tensor(args[1]), *b = tensor(args[2]), *sb = tensor(args[3]);
+    if (!a || !b || !a->is_cuda() || a->dim() < 1 || b->dim() != 2 || code_of(*a) < 0 || b->scalar_type() != a->scalar_type()) Py_RETURN_NONE;
+    const int device = a->get_device();
+    const int64_t K = a->size(-1), N = b->size(0);
+    if (!on(b, device) || !on(sa, device) || !on(sb, device) || b->size(1) != K || K < 1 || N < 1 || !is_rows(*a) || !is_rows(*b)) Py_RETURN_NONE;
+    const int64_t M = a->numel() / K;
+    if (sa->scalar_type() != at::kFloat || sb->scalar_type() != at::kFloat || !sa->is_contiguous() || !sb->is_contiguous() || sa->numel() != M || sb->numel() != N)
+        Py_RETURN_NONE;
+    const int64_t lda = M == 1 ? (K + 15) / 16 * 16 : row_stride(*a), ldb = N == 1 ? (K + 15) / 16 * 16 : row_stride(*b);
+    if (((uintptr_t)a->data_ptr() | (uintptr_t)b->data_ptr()) % 16 || (lda | ldb) % 16 || lda < K || ldb < K) Py_RETURN_NONE;
+    if (M > 0x7fffffff - 512 || N > 0x7fffffff - 512 || K > 0x7fffffff - 512) Py_RETURN_NONE;
+    const int out = (int)PyLong_AsLong(args[4]);
+    if (out == -1 && PyErr_Occurred()) return nullptr;
+    const c10::cuda::CUDAGuard guard(a->device());
+    Ctx* ctx = context_for(device);
+    if (!ctx) return nullptr;
+    at::Tensor c;
+    int rc;
+    {
+        NoGil unlocked;
+        const at::ScalarType st = out == DEERS_F16 ? at::kHalf : at::kFloat;
+        if (a->dim() == 2) {
+            c = empty_like_of({M, N}, st, *a);
+        } else {
+            std::vector<int64_t> sizes(a->sizes().begin(), a->sizes().end());
+            sizes.back() = N;
+            c = empty_like_of(sizes, st, *a);
+        }
+        std::lock_guard<std::mutex> one(ctx->mu);
+        rc = deers_b200_gemm_q8(ctx->handle, (int)M, (int)N, (int)K, code_of(*a), a->data_ptr(), lda, (const float*)sa->data_ptr(), b->data_ptr(), ldb,
+                                (const float*)sb->data_ptr(), out, c.data_ptr(), N);
+    }
+    if (rc) return fail(rc, ctx);
+    return THPVariable_Wrap(std::move(c));
+    HOST_END
+}
+
+// The cache of four tensors k, v [B,H,cap,D] e4m3 and their scales [B,H,blocks] f32; false: not one that the library takes.
+bool cache_of(PyObject* const* args, deers_cache_q8* c, int device) {
+    const at::Tensor* t[4];
+    for (int i = 0; i < 4; ++i) {
+        t[i] = tensor(args[i]);
+        if (!on(t[i], device)) return false;
+    }
+    if (t[0]->dim() != 4 || t[1]->sizes() != t[0]->sizes() || t[2]->dim() != 3 || t[3]->sizes() != t[2]->sizes()) return false;
+    const int64_t B = t[0]->size(0), H = t[0]->size(1), cap = t[0]->size(2), D = t[0]->size(3);
+    if (t[2]->size(0) != B || t[2]->size(1) != H || t[2]->size(2) != (cap + DEERS_CACHE_BLOCK - 1) / DEERS_CACHE_BLOCK || cap > 0x7fffffff) return false;
+    memset(c, 0, sizeof(*c));
+    c->B = (int)B; c->H = (int)H; c->capacity = (int)cap; c->D = (int)D;
+    c->k = t[0]->data_ptr(); c->v = t[1]->data_ptr();
+    c->k_scale = (float*)t[2]->data_ptr(); c->v_scale = (float*)t[3]->data_ptr();
+    for (int i = 0; i < 2; ++i) {
+        if (t[i]->scalar_type() != at::kFloat8_e4m3fn || t[i]->stride(3) != 1) return false;
+        if (t[2 + i]->scalar_type() != at::kFloat || (t[2 + i]->stride(2) != 1 && t[2 + i]->size(2) > 1)) return false;
+    }
+    for (int i = 0; i < 3; ++i) { c->k_strides[i] = t[0]->stride(i); c->v_strides[i] = t[1]->stride(i); }
+    for (int i = 0; i < 2; ++i) { c->k_scale_strides[i] = t[2]->stride(i); c->v_scale_strides[i] = t[3]->stride(i); }
+    // (an axis of one place never advances: any legal stride)
+    if (B == 1) c->k_strides[0] = c->v_strides[0] = 0;
+    if (H == 1) c->k_strides[1] = c->v_strides[1] = 0;
+    if (cap == 1) c->k_strides[2] = c->v_strides[2] = (D + 15) / 16 * 16;
+    return true;
+}
+inline bool places(const at::Tensor* t, int device, int64_t B) {
+    return on(t, device) && t->scalar_type() == at::kInt && t->dim() == 1 && t->size(0) == B && (B == 1 || t->stride(0) == 1);
+}
+
+// cache_taken(k_codes, v_codes, k_scale, v_scale) -> True when they are a cache that the library takes
+PyObject* cache_taken(PyObject*, PyObject* const* args, Py_ssize_t n) {
+    const at::Tensor* k = n == 4 ? tensor(args[0]) : nullptr;
+    deers_cache_q8 c;
+    if (!k || !k->is_cuda() || !cache_of(args, &c, k->get_device()) || c.D % 16 || c.D < 1 || c.D > 256 || c.B < 1 || c.H < 1 || c.capacity < 1) Py_RETURN_FALSE;
+    if (((uintptr_t)c.k | (uintptr_t)c.v) % 16) Py_RETURN_FALSE;
+    for (int i = 0; i < 3; ++i)
+        if ((c.k_strides[i] | c.v_strides[i]) % 16) Py_RETURN_FALSE;
+    Py_RETURN_TRUE;
+}
+
+// cache_append(k_codes, v_codes, k_scale, v_scale, k, v, start, count | None) -> True | None
+PyObject* cache_append(PyObject*, PyObject* const* args, Py_ssize_t n) {
+    HOST_BEGIN
+    if (n != 8) Py_RETURN_NONE;
+    const at::Tensor *k = tensor(args[4]), *v = tensor(args[5]), *start = tensor(args[6]), *count = args[7] == Py_None ? nullptr : tensor(args[7]);
+    if (!k || !v || !offerable(*k) || !v->is_cuda() || !same(*k, *v) || (k->stride(3) != 1 && k->size(3) > 1) || (v->stride(3) != 1 && v->size(3) > 1)) Py_RETURN_NONE;
+    const int device = k->get_device();
+    deers_cache_q8 c;
+    if (!cache_of(args, &c, device) || k->size(0) != c.B || k->size(1) != c.H || k->size(2) > c.capacity || k->size(3) != c.D) Py_RETURN_NONE;
+    if (!places(start, device, c.B) || (args[7] != Py_None && !places(count, device, c.B))) Py_RETURN_NONE;
+    const c10::cuda::CUDAGuard guard(k->device());
+    Ctx* ctx = context_for(device);
+    if (!ctx) return nullptr;
+    int64_t ks[4], vs[4];
+    put_strides(ks, *k); put_strides(vs, *v);
+    ks[3] = vs[3] = 1;
+    int rc;
+    {
+        NoGil unlocked;
+        std::lock_guard<std::mutex> one(ctx->mu);
+        rc = deers_b200_cache_q8_append(ctx->handle, &c, (int)k->size(2), dtype_code(*k), k->data_ptr(), ks, v->data_ptr(), vs, (const int32_t*)start->data_ptr(),
+                                        count ? (const int32_t*)count->data_ptr() : nullptr);
+    }
+    if (rc) return fail(rc, ctx);
+    Py_RETURN_TRUE;
+    HOST_END
+}
+
+// attn_decode_q8(k_codes, v_codes, k_scale, v_scale, q, lengths, scale, causal, want_lse) -> o | (o, lse) | None
+PyObject* attn_decode_q8(PyObject*, PyObject* const* args, Py_ssize_t n) {
+    HOST_BEGIN
+    if (n != 9) Py_RETURN_NONE;
+    const at::Tensor *q = tensor(args[4]), *lengths = tensor(args[5]);
+    if (!q || !offerable(*q) || q->stride(3) != 1) Py_RETURN_NONE;
+    const int device = q->get_device();
+    deers_decode_q8_desc d;
+    memset(&d, 0, sizeof(d));
+    if (!cache_of(args, &d.cache, device) || q->size(0) != d.cache.B || q->size(3) != d.cache.D || q->size(1) < 1 || d.cache.H < 1 || q->size(1) % d.cache.H ||
+        q->size(2) < 1 || q->size(2) > d.cache.capacity || !places(lengths, device, d.cache.B))
+        Py_RETURN_NONE;
+    const double scale = PyFloat_AsDouble(args[6]);
+    if (scale == -1.0 && PyErr_Occurred()) return nullptr;
+    d.H = (int)q->size(1); d.Tq = (int)q->size(2); d.dtype = dtype_code(*q); d.causal = PyObject_IsTrue(args[7]); d.scale = (float)scale;
+    const bool want_lse = PyObject_IsTrue(args[8]);
+    const c10::cuda::CUDAGuard guard(q->device());
+    Ctx* ctx = context_for(device);
+    if (!ctx) return nullptr;
+    at::Tensor o, lse, ws;
+    int rc;
+    {
+        NoGil unlocked;
+        o = empty_like_of(q->sizes(), q->scalar_type(), *q);
+        if (want_lse) lse = empty_like_of(q->sizes().slice(0, 3), at::kFloat, *q);
+        put_strides(d.q_strides, *q); put_strides(d.o_strides, o);
+        const size_t need = deers_b200_attn_decode_q8_workspace_bytes(&d);
+        if (need) ws = scratch(need, *q);
+        std::lock_guard<std::mutex> one(ctx->mu);
+        rc = deers_b200_attn_decode_q8(ctx->handle, &d, q->data_ptr(), (const int32_t*)lengths->data_ptr(), o.data_ptr(),
+                                       want_lse ? (float*)lse.data_ptr() : nullptr, need ? ws.data_ptr() : nullptr, need);
+    }
+    if (rc) return fail(rc, ctx);
+    if (!want_lse) return THPVariable_Wrap(std::move(o));
+    return wrap2(std::move(o), std::move(lse));
+    HOST_END
+}
+
 // setup(make_context, raise_status)
 PyObject* setup(PyObject*, PyObject* const* args, Py_ssize_t n) {
     if (n != 2) { PyErr_SetString(PyExc_TypeError, "setup(make_context, raise_status)"); return nullptr; }
@@ -389,6 +596,11 @@ PyMethodDef kMethods[] = {
     {"attn_decode", (PyCFunction)(void (*)())attn_decode, METH_FASTCALL, nullptr},
     {"gemm_f16", (PyCFunction)(void (*)())gemm_f16, METH_FASTCALL, nullptr},
     {"rope_pack", (PyCFunction)(void (*)())rope_pack, METH_FASTCALL, nullptr},
+    {"quantize_rows", (PyCFunction)(void (*)())quantize_rows, METH_FASTCALL, nullptr},
+    {"gemm_q8", (PyCFunction)(void (*)())gemm_q8, METH_FASTCALL, nullptr},
+    {"cache_taken", (PyCFunction)(void (*)())cache_taken, METH_FASTCALL, nullptr},
+    {"cache_append", (PyCFunction)(void (*)())cache_append, METH_FASTCALL, nullptr},
+    {"attn_decode_q8", (PyCFunction)(void (*)())attn_decode_q8, METH_FASTCALL, nullptr},
     {nullptr, nullptr, 0, nullptr}};
 
 PyModuleDef kModule = {PyModuleDef_HEAD_INIT, "_deers_host", nullptr, -1, kMethods, nullptr, nullptr, nullptr, nullptr};

@@ -56,7 +56,7 @@ enum {
     DEERS_ERR_DEVICE = 9       /* device is not an sm_100 part                          */
 };
 
-enum { DEERS_F16 = 0, DEERS_F32 = 1 };
+enum { DEERS_F16 = 0, DEERS_F32 = 1, DEERS_I8 = 2, DEERS_E4M3 = 3 };   /* the last two: codes of the 8-bit operators only */
 
 /*
  * One attention problem.  Mirrors the arguments the reference passes down its
@@ -440,6 +440,79 @@ int deers_b200_cross_entropy_fwd(deers_ctx* ctx, int64_t rows, int64_t vocab, co
 int deers_b200_cross_entropy_bwd(deers_ctx* ctx, int64_t rows, int64_t vocab, const float* logits, int64_t ld,
                                  const int64_t* targets, const float* lse, float upstream, float* dlogits,
                                  int64_t ld_dlogits);
+
+/*
+ * A block of cached decoding in 8 bits: rows of activations as codes with a scale each, products of them with an 8-bit weight, a
+ * key / value cache of codes, and the attention that reads it.  No counterpart in the reference, whose storage types are f16, bf16 and f32
+ * (`src/dtype.rs:14-21`) and whose sampling loop keeps no cache; they stand beside deers_b200_rmsnorm_fwd, deers_b200_gemm_f16 and
+ * deers_b200_attn_decode for a model that is served: a step reads the weights and the cache once, so half the bytes are half the time.
+ * Everything is enqueued on the context's stream; no allocation, no synchronisation; inference only, no gradients.
+ *
+ * quantize_rows   h = x + residual (rounded to dtype and written to sum), or x when residual is NULL, or max(x, 0)^2 with relu_squared
+ *                 (what stands between the products of the MLP, `src/models/gpt.rs:194-196`);
+ *                 y = h / sqrt(mean(h*h) + eps) with norm (`src/nn.rs:244-251`), else h;
+ *                 scale[row] = max|y| / Q, codes = nearest(y / scale), ties to even; Q = 127 (DEERS_I8) or 448 (DEERS_E4M3).
+ *                 Codes are the nearest to the exact quotient.  A row of zeros has scale 0; a row with an infinity or a NaN scale NaN and
+ *                 codes 0.  x, residual and sum: any row stride, sum may be x or residual; codes: rows on 16-byte boundaries (ld_codes a
+ *                 multiple of 16), columns behind C are left as they are.
+ */
+typedef struct deers_quantize_desc {
+    int64_t rows;
+    int32_t C;
+    int32_t dtype;            /* of x, residual and sum: DEERS_F16 / DEERS_F32 */
+    int32_t code;             /* DEERS_I8 / DEERS_E4M3 */
+    int32_t norm, relu_squared;
+    double eps;
+    int64_t ld_x, ld_residual, ld_sum, ld_codes;
+} deers_quantize_desc;
+int deers_b200_quantize_rows(deers_ctx* ctx, const deers_quantize_desc* desc, const void* x, const void* residual, void* sum, void* codes,
+                             float* scale);
+
+/*
+ * c[m, n] = a_scale[m] * b_scale[n] * sum_k a[m, k] b[n, k]: rows of codes times a weight laid out [out_features, in_features], both K
+ * contiguous and of one code type.  int8 sums are exact (K <= 131072); e4m3 sums are f32.  c is rounded once, to out_dtype (DEERS_F16 / DEERS_F32).
+ * a, b: 16-byte aligned, lda and ldb multiples of 16; c: any leading dimension (16-byte stores where rows allow).
+ */
+int deers_b200_gemm_q8(deers_ctx* ctx, int32_t M, int32_t N, int32_t K, int32_t code, const void* a, int64_t lda, const float* a_scale,
+                       const void* b, int64_t ldb, const float* b_scale, int32_t out_dtype, void* c, int64_t ldc);
+
+/*
+ * A key / value cache of e4m3 codes [B,H,capacity,D] (strides in elements, inner stride 1, the others multiples of 16) with an f32 scale for every
+ * DEERS_CACHE_BLOCK tokens of a head [B,H,ceil(capacity / DEERS_CACHE_BLOCK)] (strides of b and h).  D a multiple of 16, at most 256.
+ * cache_q8_append writes row t of k and v [B,H,T,D] (f16 or f32, inner stride 1) at place start[b] + t of sequence b, for t < count[b] (T when
+ * count is NULL); start and count are device arrays, so that a captured step serves every length.  Of a block that gets rows,
+ *     scale' = max(scale if the block holds rows before start[b], max|new rows| * (1 / 448 in f32))
+ * and where that is larger than scale the block's earlier rows are rounded again.  Nothing else changes: rows behind the last one stay as
+ * they are, and appending the same rows again changes nothing.  An infinity or a NaN is stored as NaN and takes no part in the scale.  Rows outside of
+ * the cache are left out and reported by the next deers_b200_sync (DEERS_ERR_KERNEL).
+ */
+enum { DEERS_CACHE_BLOCK = 32 };
+typedef struct deers_cache_q8 {
+    int32_t B, H, capacity, D;
+    void* k; void* v;
+    float* k_scale; float* v_scale;
+    int64_t k_strides[3], v_strides[3];               /* (b, h, t) */
+    int64_t k_scale_strides[2], v_scale_strides[2];   /* (b, h) */
+} deers_cache_q8;
+int deers_b200_cache_q8_append(deers_ctx* ctx, const deers_cache_q8* cache, int32_t T, int32_t dtype, const void* k, const int64_t* k_strides,
+                               const void* v, const int64_t* v_strides, const int32_t* start, const int32_t* count);
+
+/*
+ * Decode-time attention over such a cache: as deers_b200_attn_decode, but sequence b has lengths[b] rows (a device array; the Tq newest of
+ * them belong to the queries), and H query heads share the cache's heads: head h reads head h / (H / cache.H).  Query i sees keys
+ * j < lengths[b] - (Tq - 1 - i) when causal, all lengths[b] otherwise; one that sees none has o = 0 and lse = -infinity.  q, o [B,H,Tq,D] f16 or
+ * f32 with unit inner stride; lse [B,H,Tq] f32, may be NULL.  Sums and softmax are f32.  A length outside of [0, capacity] is taken as the nearest
+ * inside and reported by the next deers_b200_sync.  Workspace: deers_b200_attn_decode_q8_workspace_bytes(desc), 0 for most calls.
+ */
+typedef struct deers_decode_q8_desc {
+    deers_cache_q8 cache;
+    int32_t H, Tq, dtype, causal;
+    float scale;
+    int64_t q_strides[4], o_strides[4];
+} deers_decode_q8_desc;
+size_t deers_b200_attn_decode_q8_workspace_bytes(const deers_decode_q8_desc* desc);
+int deers_b200_attn_decode_q8(deers_ctx* ctx, const deers_decode_q8_desc* desc, const void* q, const int32_t* lengths, void* o, float* lse,
+                              void* workspace, size_t workspace_bytes);
 
 /*
  * The GPT of `src/models/gpt.rs` as one device-resident object: parameters, gradients, AdamW moments and
