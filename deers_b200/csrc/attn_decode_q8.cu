@@ -60,14 +60,20 @@ __device__ __forceinline__ uint32_t transposed(uint32_t a) {
     return d;
 }
 template <int BYTES>
-__device__ __forceinline__ void copy_in(uint32_t dst, const uint8_t* src, bool there) {
-    const int n = there ? BYTES : 0;
+__device__ __forceinline__ void copy_in(uint32_t dst, const uint8_t* src, uint32_t n) {
     if constexpr (BYTES == 16) asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(n) : "memory");
     else asm volatile("cp.async.ca.shared.global [%0], [%1], 8, %2;" ::"r"(dst), "l"(src), "r"(n) : "memory");
 }
 __device__ __forceinline__ void copies_end_group() { asm volatile("cp.async.commit_group;" ::: "memory"); }
 template <int N>
 __device__ __forceinline__ void copies_wait() { asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory"); }
+
+// 2^x for x <= 0 (results below 2^-126 are zero).
+__device__ __forceinline__ float power2(float x) {
+    float y;
+    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+    return y;
+}
 
 __device__ __forceinline__ void put(float* p, float v) { *p = v; }
 __device__ __forceinline__ void put(__half* p, float v) { *p = __float2half_rn(v); }
@@ -78,14 +84,14 @@ struct Shape {
     static constexpr int KC = DP / 64;                           // 16-byte pieces of a key that a lane owns: at 16 * (lane % 4 + 4 c)
     static constexpr int VB = DP >= 128 ? 16 : 8;                // bytes of a piece of V: at VB * (lane / 4 + 8 c)
     static constexpr int VC = DP / 8 / VB;
-    static constexpr int STAGES = DP == 256 ? 2 : DP == 128 ? 3 : 4;
+    static constexpr int STAGES = DP == 64 ? 4 : 2;
     static constexpr int STAGE_BYTES = 32 * 2 * DP;              // 32 keys: every byte of them is some lane's
     static constexpr int RING = DQ_WARPS * STAGES * STAGE_BYTES;
     static constexpr int ROWS = 8 * NT;
     static constexpr int OS = DP + 4;                            // row of partial results: O, then maximum and sum
     static constexpr int MERGE = DQ_WARPS * ROWS * OS * 4;
     static constexpr int PART = ROWS * OS * 4;
-    static constexpr int SMEM = (RING > MERGE ? RING : MERGE) + PART;
+    static constexpr int SMEM = RING > MERGE + PART ? RING : MERGE + PART;         // (the ring has been read when the warps meet)
 };
 
 enum DecodeQ8End { DQ_ONE_CHUNK = 0, DQ_CLUSTER = 1, DQ_TO_WORKSPACE = 2 };
@@ -116,31 +122,50 @@ __global__ void __launch_bounds__(32 * DQ_WARPS) decode_q8_kernel(const DecodeQ8
     uint8_t* ring = smem + warp * (S::STAGES * S::STAGE_BYTES);
     const uint32_t ring_u = (uint32_t)__cvta_generic_to_shared(ring) + lane * 16;
     const uint32_t vring_u = (uint32_t)__cvta_generic_to_shared(ring) + 32 * DP + lane * S::VB;
+    // This lane's keys of a block: 8 r + g of K; 2t, 2t + 1, 2t + 8, 2t + 9 of either half of V.
+    const auto k_key = [&](int r) { return 8 * r + g; };
+    const auto v_key = [&](int r) { return (r >> 2) * 16 + ((r >> 1) & 1) * 8 + 2 * t + (r & 1); };
+    uint32_t k_at[4], v_at[8], k_size[S::KC], v_size[S::VC];     // their places relative to the block's, and the bytes that a piece has
+#pragma unroll
+    for (int r = 0; r < 4; ++r) k_at[r] = (uint32_t)k_key(r) * (uint32_t)p.sk[2] + 16 * t;
+#pragma unroll
+    for (int r = 0; r < 8; ++r) v_at[r] = (uint32_t)v_key(r) * (uint32_t)p.sv[2] + S::VB * g;
+#pragma unroll
+    for (int c = 0; c < S::KC; ++c) k_size[c] = 16 * (t + 4 * c) < p.D ? 16 : 0;
+#pragma unroll
+    for (int c = 0; c < S::VC; ++c) v_size[c] = S::VB * (g + 8 * c) < p.D ? S::VB : 0;
     // Fetches block `blk` into stage s.  Keys behind the last are zeros: what lies there belongs to nobody.
     auto fetch = [&](int blk, int s) {
         if (blk < blk1) {
-            const int j0 = blk * 32;
+            const uint8_t* kp = kb + (long long)blk * 32 * p.sk[2];
+            const uint8_t* vp = vb + (long long)blk * 32 * p.sv[2];
+            const int left = len - blk * 32;                     // keys from here on
+            if (left >= 32) {
 #pragma unroll
-            for (int r = 0; r < 4; ++r) {
-                const int j = j0 + 8 * r + g;
-                const uint8_t* src = kb + (long long)min(j, len - 1) * p.sk[2];
+                for (int r = 0; r < 4; ++r)
 #pragma unroll
-                for (int c = 0; c < S::KC; ++c) {
-                    const int d = 16 * (t + 4 * c);
-                    const bool there = j < len && d < p.D;
-                    copy_in<16>(ring_u + s * S::STAGE_BYTES + (r * S::KC + c) * 512, there ? src + d : kb, there);
-                }
-            }
+                    for (int c = 0; c < S::KC; ++c)
+                        copy_in<16>(ring_u + s * S::STAGE_BYTES + (r * S::KC + c) * 512, kp + k_at[r] + (DP > 64 && k_size[c] ? 64 * c : 0), k_size[c]);
 #pragma unroll
-            for (int r = 0; r < 8; ++r) {                        // keys 2t, 2t + 1, 2t + 8, 2t + 9 of either half
-                const int j = j0 + (r >> 2) * 16 + ((r >> 1) & 1) * 8 + 2 * t + (r & 1);
-                const uint8_t* src = vb + (long long)min(j, len - 1) * p.sv[2];
+                for (int r = 0; r < 8; ++r)
 #pragma unroll
-                for (int c = 0; c < S::VC; ++c) {
-                    const int d = S::VB * (g + 8 * c);
-                    const bool there = j < len && d < p.D;
-                    copy_in<S::VB>(vring_u + s * S::STAGE_BYTES + (r * S::VC + c) * (32 * S::VB), there ? src + d : vb, there);
-                }
+                    for (int c = 0; c < S::VC; ++c)
+                        copy_in<S::VB>(vring_u + s * S::STAGE_BYTES + (r * S::VC + c) * (32 * S::VB), vp + v_at[r] + (S::VC > 1 && v_size[c] ? 128 * c : 0), v_size[c]);
+            } else {
+#pragma unroll
+                for (int r = 0; r < 4; ++r)
+#pragma unroll
+                    for (int c = 0; c < S::KC; ++c) {
+                        const uint32_t n = k_key(r) < left ? k_size[c] : 0;
+                        copy_in<16>(ring_u + s * S::STAGE_BYTES + (r * S::KC + c) * 512, n ? kp + k_at[r] + 64 * c : kb, n);
+                    }
+#pragma unroll
+                for (int r = 0; r < 8; ++r)
+#pragma unroll
+                    for (int c = 0; c < S::VC; ++c) {
+                        const uint32_t n = v_key(r) < left ? v_size[c] : 0;
+                        copy_in<S::VB>(vring_u + s * S::STAGE_BYTES + (r * S::VC + c) * (32 * S::VB), n ? vp + v_at[r] + 128 * c : vb, n);
+                    }
             }
         }
         copies_end_group();
@@ -227,9 +252,12 @@ __global__ void __launch_bounds__(32 * DQ_WARPS) decode_q8_kernel(const DecodeQ8
     }
 
     int stage = 0;
+    float ks_next = 0.f, vs_next = 0.f;                          // scales of the next round's block
+    if (blk0 + warp < blk1) { ks_next = ksl[blk0 + warp]; vs_next = vsl[blk0 + warp]; }
 #pragma unroll 1
     for (int blk = blk0 + warp; blk < blk1; blk += DQ_WARPS) {
-        const float ks = ksl[blk], vs = vsl[blk];
+        const float ks = ks_next, vs = vs_next;
+        if (blk + DQ_WARPS < blk1) { ks_next = ksl[blk + DQ_WARPS]; vs_next = vsl[blk + DQ_WARPS]; }
         copies_wait<S::STAGES - 2>();
         {
             const int into = stage == 0 ? S::STAGES - 1 : stage - 1;         // the stage that the last round has read
@@ -289,17 +317,23 @@ __global__ void __launch_bounds__(32 * DQ_WARPS) decode_q8_kernel(const DecodeQ8
 #pragma unroll
                 for (int mt = 0; mt < 2; ++mt)
 #pragma unroll
-                    for (int y = 0; y < 2; ++y) {
-                        float z = s[nt][mt][2 * y + x] * f;
-                        if (edge && blk * 32 + mt * 16 + y * 8 + g >= lim[nt][x]) z = -INFINITY;
-                        s[nt][mt][2 * y + x] = z;
-                        mx = fmaxf(mx, z);
-                    }
+                    for (int y = 0; y < 2; ++y) s[nt][mt][2 * y + x] *= f;
+                if (edge) {
+#pragma unroll
+                    for (int mt = 0; mt < 2; ++mt)
+#pragma unroll
+                        for (int y = 0; y < 2; ++y)
+                            if (blk * 32 + mt * 16 + y * 8 + g >= lim[nt][x]) s[nt][mt][2 * y + x] = -INFINITY;
+                }
+#pragma unroll
+                for (int mt = 0; mt < 2; ++mt)
+#pragma unroll
+                    for (int y = 0; y < 2; ++y) mx = fmaxf(mx, s[nt][mt][2 * y + x]);
 #pragma unroll
                 for (int off = 4; off <= 16; off *= 2) mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, off));
                 // (-inf: nothing seen so far, or NaN alone, which have to reach the sums)
                 const float ms = mx == -INFINITY ? 0.f : mx;
-                fac[nt][x] = exp2f(m[nt][x] - ms);
+                fac[nt][x] = power2(m[nt][x] - ms);
                 moved |= mx != m[nt][x];
                 m[nt][x] = mx;
                 l[nt][x] *= fac[nt][x];
@@ -307,7 +341,7 @@ __global__ void __launch_bounds__(32 * DQ_WARPS) decode_q8_kernel(const DecodeQ8
                 for (int mt = 0; mt < 2; ++mt)
 #pragma unroll
                     for (int y = 0; y < 2; ++y) {
-                        const float pj = exp2f(s[nt][mt][2 * y + x] - ms);
+                        const float pj = power2(s[nt][mt][2 * y + x] - ms);
                         l[nt][x] += pj;
                         s[nt][mt][2 * y + x] = pj;
                     }
@@ -437,7 +471,7 @@ __global__ void __launch_bounds__(32 * DQ_WARPS) decode_q8_kernel(const DecodeQ8
             for (int off = 4; off <= 16; off *= 2) l[nt][x] += __shfl_xor_sync(0xffffffffu, l[nt][x], off);
     __syncthreads();                                             // every ring has been read
     float* meet = reinterpret_cast<float*>(smem);
-    float* part = reinterpret_cast<float*>(smem + (S::RING > S::MERGE ? S::RING : S::MERGE));
+    float* part = reinterpret_cast<float*>(smem + S::MERGE);
     {
         float* mine = meet + warp * S::ROWS * S::OS;
         const float down = vref * (1.0f / DQ_UP);

@@ -24,12 +24,14 @@ struct AppendParams {
 
 __device__ __forceinline__ float as_f(__half v) { return __half2float(v); }
 __device__ __forceinline__ float as_f(float v) { return v; }
+__device__ __forceinline__ __half not_a_number(__half) { return __ushort_as_half(0x7e00); }
+__device__ __forceinline__ float not_a_number(float) { return __uint_as_float(0x7fc00000u); }
 
-// 32 * NW threads own a token block; NP pieces of four values each stay in registers.
-template <typename T, bool VEC, int NW, int NP>
+// 32 * NW threads own a token block, LR threads a row of it, eight values each; NP rows of a thread stay in registers.
+template <typename T, bool VEC, int LR, int NW, int NP>
 __global__ void __launch_bounds__(128) append_q8_kernel(const AppendParams p) {
     chain_begin();
-    constexpr int NT = 32 * NW, PER = 128 / NT;                  // groups of a block of threads
+    constexpr int NT = 32 * NW, PER = 128 / NT, STEP = NT / LR;  // groups of a block of threads; rows at a time
     const int tid = threadIdx.x % NT, warp = threadIdx.x / 32;
     const int h = blockIdx.y * PER + threadIdx.x / NT, b = blockIdx.z >> 1, kv = blockIdx.z & 1;
     const bool mine = h < p.H;                                   // (with NW == 4 the whole block)
@@ -44,63 +46,71 @@ __global__ void __launch_bounds__(128) append_q8_kernel(const AppendParams p) {
     const int blk = begin / q8::BLOCK + blockIdx.x, first = blk * q8::BLOCK;
     const int lo = max(begin, first), hi = min(begin + n, first + q8::BLOCK);
     if (lo >= hi) return;
-    const T* src = static_cast<const T*>(p.src[kv]) + b * p.ss[kv][0] + h * p.ss[kv][1] + (long long)(lo - begin) * p.ss[kv][2];
     uint8_t* codes = p.codes[kv] + b * p.sc[kv][0] + h * p.sc[kv][1];
     float* scale_at = p.scale[kv] + b * p.sl[kv][0] + h * p.sl[kv][1] + blk;
-    const long long st = p.ss[kv][2], sc = p.sc[kv][2];
-    const int per_row = p.D / 4, pieces = (hi - lo) * per_row;
+    const int row = tid / LR, col = tid % LR * 8, rows = col < p.D ? hi - lo - row : 0;      // this thread's: row, row + STEP, ..
+    const T* src = static_cast<const T*>(p.src[kv]) + b * p.ss[kv][0] + h * p.ss[kv][1] + (long long)(lo - begin + row) * p.ss[kv][2] + col;
     const float was = begin > first ? *scale_at : 0.f;
-    float v[NP][4];
-    unsigned top = 0;
+    T v[NP][8];
 #pragma unroll
     for (int i = 0; i < NP; ++i) {
-        const int at = tid + i * NT;
-        if (at < pieces) {
-            const T* s = src + at / per_row * st + at % per_row * 4;
+        if (i * STEP < rows) {
+            const T* s = src + i * STEP * p.ss[kv][2];
             if constexpr (VEC) {
-                T raw[4];
-                if constexpr (sizeof(T) == 2) *reinterpret_cast<uint2*>(raw) = *reinterpret_cast<const uint2*>(s);
-                else *reinterpret_cast<uint4*>(raw) = *reinterpret_cast<const uint4*>(s);
 #pragma unroll
-                for (int e = 0; e < 4; ++e) v[i][e] = as_f(raw[e]);
+                for (int w = 0; w < (int)sizeof(T) / 2; ++w) reinterpret_cast<uint4*>(v[i])[w] = reinterpret_cast<const uint4*>(s)[w];
             } else {
 #pragma unroll
-                for (int e = 0; e < 4; ++e) v[i][e] = as_f(s[e]);
+                for (int e = 0; e < 8; ++e) v[i][e] = s[e];
             }
         }
     }
+    auto most = [&]() {                                          // the group's largest |value|, NaN passed over
+        float top = 0.f;
 #pragma unroll
-    for (int i = 0; i < NP; ++i) {
-        if (tid + i * NT < pieces) {
+        for (int i = 0; i < NP; ++i) {
+            if (i * STEP < rows) {
 #pragma unroll
-            for (int e = 0; e < 4; ++e) {
-                const unsigned bits = __float_as_uint(v[i][e]) & 0x7fffffffu;
-                if (bits < 0x7f800000u) top = max(top, bits);
-                else v[i][e] = __uint_as_float(0x7fc00000u);
+                for (int e = 0; e < 8; e += 4) {
+                    float f[4];
+                    q8::four(v[i] + e, f);
+                    q8::look_at(top, f);
+                }
             }
         }
-    }
 #pragma unroll
-    for (int off = 16; off >= 1; off >>= 1) top = max(top, __shfl_xor_sync(0xffffffffu, top, off));
-    if constexpr (NW > 1) {
-        __shared__ unsigned s_top[4];
-        if ((threadIdx.x & 31) == 0) s_top[warp] = top;
-        __syncthreads();
+        for (int off = 16; off >= 1; off >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, off));
+        if constexpr (NW > 1) {
+            __shared__ float s_top[4];
+            __syncthreads();
+            if ((threadIdx.x & 31) == 0) s_top[warp] = top;
+            __syncthreads();
 #pragma unroll
-        for (int w = 0; w < NW; ++w) top = max(top, s_top[w]);
-    } else {
-        __syncwarp();                                            // every lane has read the old scale
+            for (int w = 0; w < NW; ++w) top = fmaxf(top, s_top[w]);
+        } else {
+            __syncwarp();                                        // every lane has read the old scale
+        }
+        return top;
+    };
+    const float inf = __uint_as_float(0x7f800000u);
+    float top = most();
+    if (!(top < inf)) {                                          // infinities are no part of the scale, and are stored as NaN
+#pragma unroll
+        for (int i = 0; i < NP; ++i)
+#pragma unroll
+            for (int e = 0; e < 8; ++e)
+                if (fabsf(as_f(v[i][e])) == inf) v[i][e] = not_a_number(v[i][e]);
+        top = most();
     }
-    const float fresh = __uint_as_float(top) * (1.0f / q8::MOST_E4M3);
+    const float fresh = top * (1.0f / q8::MOST_E4M3);
     const bool grown = fresh > was;
     const float scale = grown ? fresh : was;
-    const float inf = __uint_as_float(0x7f800000u);
     if (tid == 0) *scale_at = scale;
     if (grown && begin > first) {                                // the earlier rows, 16 bytes at a time
-        const float again = was / scale;
+        const q8::Factors again = q8::factors(was, scale, q8::den_is_far(scale) || !(was > 1e-20f));
         const int per16 = p.D / 16, old16 = (begin - first) * per16;
         for (int at = tid; at < old16; at += NT) {
-            uint4* c = reinterpret_cast<uint4*>(codes + (first + at / per16) * sc + at % per16 * 16);
+            uint4* c = reinterpret_cast<uint4*>(codes + (first + at / per16) * p.sc[kv][2] + at % per16 * 16);
             const uint4 w = *c;
             const uint32_t in[4] = {w.x, w.y, w.z, w.w};
             uint32_t out[4];
@@ -108,32 +118,44 @@ __global__ void __launch_bounds__(128) append_q8_kernel(const AppendParams p) {
             for (int k = 0; k < 4; ++k) {
                 float f[4];
                 q8::e4m3_values(in[k], f);
-                out[k] = q8::codes_of<false>(f, again, was, scale, false);
+                out[k] = q8::codes_of<false>(f, again, was, scale);
             }
             *c = make_uint4(out[0], out[1], out[2], out[3]);
         }
     }
-    const float r = scale > 0.f ? 1.0f / scale : 0.f;
-    const bool wide = !(r < inf);
+    const float den = scale > 0.f ? scale : 1.0f;
+    const q8::Factors factors = q8::factors(1.0f, den, q8::den_is_far(den));
+    uint8_t* to = codes + (lo + row) * p.sc[kv][2] + col;
 #pragma unroll
     for (int i = 0; i < NP; ++i) {
-        const int at = tid + i * NT;
-        if (at < pieces) *reinterpret_cast<uint32_t*>(codes + (lo + at / per_row) * sc + at % per_row * 4) = q8::codes_of<false>(v[i], r, 1.0f, scale > 0.f ? scale : 1.0f, wide);
+        if (i * STEP < rows) {
+            uint32_t c[2];
+#pragma unroll
+            for (int k = 0; k < 2; ++k) {
+                float f[4];
+                q8::four(v[i] + 4 * k, f);
+                c[k] = q8::codes_of<false>(f, factors, 1.0f, den);
+            }
+            *reinterpret_cast<uint2*>(to + i * STEP * p.sc[kv][2]) = make_uint2(c[0], c[1]);
+        }
     }
 }
 
-template <typename T, bool VEC>
-int append_launch(deers_ctx* ctx, const AppendParams& p, int B) {
+// A warp for a token block that gets few rows, four warps otherwise.
+template <typename T, bool VEC, int LR>
+int append_widths(deers_ctx* ctx, const AppendParams& p, int B) {
     // token blocks that T rows can touch from any place
     const unsigned blocks = p.T < 2 ? 1u : (unsigned)((p.T - 2) / q8::BLOCK + 2);
-    const int rows = p.T < q8::BLOCK ? p.T : q8::BLOCK, pieces = rows * p.D / 4;         // of a token block, at most
     KernelTimerScope ts(ctx, DEERS_K_DECODE);
     const dim3 warps(blocks, (unsigned)((p.H + 3) / 4), 2u * B), whole(blocks, (unsigned)p.H, 2u * B);
-    if (pieces <= 64) DEERS_CUDA_TRY(ctx, launch_chained(ctx, append_q8_kernel<T, VEC, 1, 2>, warps, 128, 0, 1, p));
-    else if (pieces <= 256) DEERS_CUDA_TRY(ctx, launch_chained(ctx, append_q8_kernel<T, VEC, 1, 8>, warps, 128, 0, 1, p));
-    else if (pieces <= 1024) DEERS_CUDA_TRY(ctx, launch_chained(ctx, append_q8_kernel<T, VEC, 4, 8>, whole, 128, 0, 1, p));
-    else DEERS_CUDA_TRY(ctx, launch_chained(ctx, append_q8_kernel<T, VEC, 4, 16>, whole, 128, 0, 1, p));
+    if (p.T <= 32 / LR) DEERS_CUDA_TRY(ctx, launch_chained(ctx, append_q8_kernel<T, VEC, LR, 1, 1>, warps, 128, 0, 1, p));
+    else if (p.T <= 128 / LR) DEERS_CUDA_TRY(ctx, launch_chained(ctx, append_q8_kernel<T, VEC, LR, 1, 4>, warps, 128, 0, 1, p));
+    else DEERS_CUDA_TRY(ctx, launch_chained(ctx, append_q8_kernel<T, VEC, LR, 4, LR / 4>, whole, 128, 0, 1, p));
     return DEERS_OK;
+}
+template <typename T, bool VEC>
+int append_launch(deers_ctx* ctx, const AppendParams& p, int B) {
+    return p.D <= 64 ? append_widths<T, VEC, 8>(ctx, p, B) : p.D <= 128 ? append_widths<T, VEC, 16>(ctx, p, B) : append_widths<T, VEC, 32>(ctx, p, B);
 }
 
 }  // namespace
@@ -141,7 +163,8 @@ int append_launch(deers_ctx* ctx, const AppendParams& p, int B) {
 int deers_check_cache(const deers_cache_q8* c) {
     if (!c) return DEERS_ERR_NULL;
     if (c->B < 1 || c->H < 1 || c->capacity < 1 || c->D < 1) return DEERS_ERR_SHAPE;
-    if (c->D % 16 || c->D > 256 || c->B > 32767 || c->H > 65535 || c->capacity > (1 << 24)) return DEERS_ERR_UNSUPPORTED;
+    if (c->D % 16 || c->D > 256 || c->B > 32767 || c->H > 65535 || c->capacity > (1 << 24) || c->k_strides[2] > (1 << 26) || c->v_strides[2] > (1 << 26))
+        return DEERS_ERR_UNSUPPORTED;
     if (!c->k || !c->v || !c->k_scale || !c->v_scale) return DEERS_ERR_NULL;
     if (((uintptr_t)c->k | (uintptr_t)c->v) & 15u || ((uintptr_t)c->k_scale | (uintptr_t)c->v_scale) & 3u) return DEERS_ERR_LAYOUT;
     for (int i = 0; i < 3; ++i)
@@ -164,14 +187,13 @@ extern "C" int deers_b200_cache_q8_append(deers_ctx* ctx, const deers_cache_q8* 
     const int64_t es = dtype == DEERS_F16 ? 2 : 4;
     if (((uintptr_t)k | (uintptr_t)v) & (uintptr_t)(es - 1) || ((uintptr_t)start | (uintptr_t)count) & 3u) return DEERS_ERR_LAYOUT;
     if (k_strides[3] != 1 || v_strides[3] != 1) return DEERS_ERR_LAYOUT;
-    const int64_t al = 4 * es;                                    // four values at a time
-    bool vec = (((uintptr_t)k | (uintptr_t)v) & (uintptr_t)(al - 1)) == 0;
+    bool vec = (((uintptr_t)k | (uintptr_t)v) & 15u) == 0;
     AppendParams p;
     for (int i = 0; i < 3; ++i) {
         if (k_strides[i] < 0 || v_strides[i] < 0) return DEERS_ERR_LAYOUT;
         // (a cache whose sequences or heads are one place can be read, not written)
         if ((i == 0 ? c->B : i == 1 ? c->H : 1) > 1 && (c->k_strides[i] == 0 || c->v_strides[i] == 0)) return DEERS_ERR_LAYOUT;
-        vec = vec && ((k_strides[i] | v_strides[i]) & 3) == 0;
+        vec = vec && ((k_strides[i] | v_strides[i]) * es & 15) == 0;
         p.ss[0][i] = k_strides[i]; p.ss[1][i] = v_strides[i];
         p.sc[0][i] = c->k_strides[i]; p.sc[1][i] = c->v_strides[i];
     }

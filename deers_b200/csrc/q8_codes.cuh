@@ -3,6 +3,8 @@
 #include <cuda_fp16.h>
 #include <stdint.h>
 
+#include "f32_util.cuh"
+
 namespace q8 {
 
 constexpr float MOST_I8 = 127.0f, MOST_E4M3 = 448.0f;            // largest code
@@ -37,46 +39,108 @@ __device__ __forceinline__ float round_to_odd(double x) {
     const float f = __double2float_rz(x);
     return (double)f == x ? f : __uint_as_float(__float_as_uint(f) | 1u);
 }
-
-// Four codes worked out in 64 bits.
-static __device__ __noinline__ uint32_t exact_e4m3(float a, float b, float c, float d, float num, float den) {
-    return e4m3_of(round_to_odd((double)a * (double)num / (double)den), round_to_odd((double)b * (double)num / (double)den),
-                   round_to_odd((double)c * (double)num / (double)den), round_to_odd((double)d * (double)num / (double)den));
-}
-static __device__ __noinline__ uint32_t exact_i8(float v, float num, float den) {
-    const int q = __double2int_rn((double)v * (double)num / (double)den);
-    return (uint32_t)(q > 127 ? 127 : q < -127 ? -127 : q);
-}
-
-// Codes of four quotients v[i] * num / den, each the nearest code to the exact quotient (ties to even), given r = num / den rounded.
-// v * r is off by at most 2^-23 of itself, so a quotient whose neighbours 2^-21 to either side have one code has that code; the few others are
-// worked out in 64 bits.  So the codes follow from the operator's definition alone, not from the order of this kernel's operations.
-// wide: r does not stand for the quotient (it overflowed).
+// Four codes of quotients v * num / den worked out in 64 bits: for operands whose products leave f32.
 template <bool I8>
-__device__ __forceinline__ uint32_t codes_of(const float (&v)[4], float r, float num, float den, bool wide) {
-    constexpr float DOWN = 1.0f - 4.76837158e-7f, UP = 1.0f + 4.76837158e-7f;
-    float t[4];
+static __device__ __noinline__ uint32_t codes_far(float a, float b, float c, float d, float num, float den) {
+    const double x[4] = {(double)a * num / den, (double)b * num / den, (double)c * num / den, (double)d * num / den};
+    if constexpr (I8) {
+        uint32_t w = 0;
 #pragma unroll
-    for (int i = 0; i < 4; ++i) t[i] = v[i] * r;
+        for (int i = 0; i < 4; ++i) w |= ((uint32_t)__double2int_rn(fmin(fmax(x[i], -127.0), 127.0)) & 0xffu) << (8 * i);
+        return w;
+    }
+    return e4m3_of(round_to_odd(x[0]), round_to_odd(x[1]), round_to_odd(x[2]), round_to_odd(x[3]));
+}
+
+// Sign of |v| * num - |mid| * den, exactly: the products' rounding errors are f32 values too.  The products are next to one another, so their
+// difference is exact as well.  mid has few bits; num and den are such that nothing overflows or falls among the subnormals.
+__device__ __forceinline__ float beyond(float v, float num, float mid, float den) {
+    const float a = fabsf(v), m = fabsf(mid), p = a * num, q = m * den;
+    return (p - q) + (fmaf(a, num, -p) - fmaf(m, den, -q));
+}
+
+// Products of den with a border, or of the quotient's operands, could leave f32.
+__device__ __forceinline__ bool den_is_far(float den) { return !(den > 1e-20f && den < 1e20f); }
+
+// The factors that bring values next to their quotients v * num / den: r = num / den is off by 2^-24 of itself, and so is each of the two products that
+// follow, so the quotient lies between v * down and v * up.  far: neither says anything, and nothing is between them.
+struct Factors { float down, up; };
+__device__ __forceinline__ Factors factors(float num, float den, bool far) {
+    const float r = num / den;
+    return far ? Factors{0.f, __uint_as_float(0x7f800000u)} : Factors{r * (1.0f - 2.38418579e-7f), r * (1.0f + 2.38418579e-7f)};       // 2^-22
+}
+
+// Of values whose quotient may lie on either side of a border, the code by an exact comparison with it; ties to even.
+static __device__ __noinline__ uint32_t decide_e4m3(uint32_t lo, uint32_t hi, float v0, float v1, float v2, float v3, float num, float den) {
+    if (den_is_far(den) || !(num > 1e-20f)) return codes_far<false>(v0, v1, v2, v3, num, den);
+    const float v[4] = {v0, v1, v2, v3};
+    float a[4], b[4];
+    e4m3_values(lo, a);
+    e4m3_values(hi, b);
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+        const uint32_t mask = 0xffu << (8 * i);
+        if ((lo ^ hi) & mask) {                                  // neighbours of one sign, hi the larger
+            const float side = beyond(v[i], num, 0.5f * (a[i] + b[i]), den);
+            if (side > 0.f || (side == 0.f && (lo >> (8 * i)) & 1u)) lo = (lo & ~mask) | (hi & mask);
+        }
+    }
+    return lo;
+}
+static __device__ __noinline__ uint32_t decide_i8(float v0, float v1, float v2, float v3, float num, float den) {
+    if (den_is_far(den)) return codes_far<true>(v0, v1, v2, v3, num, den);
+    const float v[4] = {v0, v1, v2, v3};
+    uint32_t w = 0;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+        const float low = fminf(floorf(fabsf(v[i] * (num / den))), 126.f);           // the two sizes: low, low + 1 (or the quotient is whole)
+        const float side = beyond(v[i], num, low + 0.5f, den);
+        int size = (int)low + (side > 0.f || (side == 0.f && ((int)low & 1)) ? 1 : 0);
+        w |= ((uint32_t)(v[i] < 0.f ? -size : size) & 0xffu) << (8 * i);
+    }
+    return w;
+}
+
+// Codes of four quotients v[i] * num / den, each the nearest code to the exact quotient (ties to even).  Where both bounds of a quotient have one
+// code, that is it; the few others are decided exactly, so the codes follow from the operator's definition alone, not from the order of this
+// kernel's operations.  (f16 values meet borders often: three normal ones in ten thousand.)
+template <bool I8>
+__device__ __forceinline__ uint32_t codes_of(const float (&v)[4], const Factors& f, float num, float den) {
+    const uint64_t v01 = pack_f32x2(v[0], v[1]), v23 = pack_f32x2(v[2], v[3]), up = pack_f32x2(f.up, f.up);
+    float u[4];
+    unpack_f32x2(mul2(v01, up), u[0], u[1]);
+    unpack_f32x2(mul2(v23, up), u[2], u[3]);
     if constexpr (I8) {
         constexpr float MAGIC = 12582912.0f;                      // 1.5 * 2^23: the sum's low bits are the nearest whole number
         uint32_t c[4];
-        bool near = wide;                                        // (of 127 the error is 2^-16: borders are looked for 2^-13 to either side)
+        bool near = false;                                       // (of 127 the factor is off by 2^-14.6 at most: borders are looked for 2^-13 to either side)
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
-            const float m = t[i] + MAGIC;
-            near |= !(fabsf(t[i] - (m - MAGIC)) < 0.4998f);
+            const float m = u[i] + MAGIC;
+            near |= !(fabsf(u[i] - (m - MAGIC)) < 0.49985f);
             c[i] = __float_as_uint(m);
         }
-        if (near) {
-#pragma unroll
-            for (int i = 0; i < 4; ++i) c[i] = exact_i8(v[i], num, den);
-        }
+        if (near) return decide_i8(v[0], v[1], v[2], v[3], num, den);
         return __byte_perm(__byte_perm(c[0], c[1], 0x0040), __byte_perm(c[2], c[3], 0x0040), 0x5410);
     } else {
-        const uint32_t lo = e4m3_of(t[0] * DOWN, t[1] * DOWN, t[2] * DOWN, t[3] * DOWN), hi = e4m3_of(t[0] * UP, t[1] * UP, t[2] * UP, t[3] * UP);
-        return lo == hi && !wide ? lo : exact_e4m3(v[0], v[1], v[2], v[3], num, den);
+        const uint64_t down = pack_f32x2(f.down, f.down);
+        float d[4];
+        unpack_f32x2(mul2(v01, down), d[0], d[1]);
+        unpack_f32x2(mul2(v23, down), d[2], d[3]);
+        const uint32_t lo = e4m3_of(d[0], d[1], d[2], d[3]), hi = e4m3_of(u[0], u[1], u[2], u[3]);
+        return lo == hi ? lo : decide_e4m3(lo, hi, v[0], v[1], v[2], v[3], num, den);
     }
+}
+
+// |v| into a running maximum that passes over NaN; the four values as f32.
+__device__ __forceinline__ void look_at(float& top, const float (&v)[4]) { top = fmaxf(fmaxf(top, fmaxf(fabsf(v[0]), fabsf(v[1]))), fmaxf(fabsf(v[2]), fabsf(v[3]))); }
+__device__ __forceinline__ void four(const float* v, float (&f)[4]) {
+#pragma unroll
+    for (int e = 0; e < 4; ++e) f[e] = v[e];
+}
+__device__ __forceinline__ void four(const __half* v, float (&f)[4]) {
+    const float2 a = __half22float2(__halves2half2(v[0], v[1])), b = __half22float2(__halves2half2(v[2], v[3]));
+    f[0] = a.x; f[1] = a.y; f[2] = b.x; f[3] = b.y;
 }
 
 }  // namespace q8

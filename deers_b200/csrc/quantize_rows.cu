@@ -8,7 +8,11 @@
 // the row (its maximum and its sum of squares meet in one exchange), codes from the registers that hold it; the norm's rows in f32 and the
 // pass that would quantise them never exist.  Codes are the nearest to the exact quotient (q8_codes.cuh).
 // A row of zeros has scale 0.  A row with an infinity or a NaN has scale NaN and codes 0: every product of it is NaN, as it is of the norm.
-// Bound: HBM, 7 bytes an element with f16 and a residual, 13 with f32.
+// Bound: HBM, 7 bytes an element with f16 and a residual, 13 with f32: 16384 x 2048 f16 41 us (5.7 TB/s, 0.88 of the copy rate), 8192 x 4096 f32 79 us (0.85).
+// What it took: a row on as few threads as hold it in 40 registers, so that an SM has 1536 (48 -> 42 us; at 60 registers loads of too few rows
+// were in flight); borders between codes decided by exact products instead of a 64-bit division for every value next to one (relative to
+// that 51 -> 48, and new keys and values, cache_q8.cu, 141 -> 43); units that neighbouring threads interleave where rows start on no 16-byte
+// boundary (4096 x 4100 f16 106 -> 39 us).
 #include "common.cuh"
 #include "q8_codes.cuh"
 
@@ -20,52 +24,66 @@ struct QuantParams {
     long long rows;
     int C;
     float eps, inv_n;
-    int norm, relu2;
+    int norm;
 };
 
-template <typename T> struct Piece;                              // 16 bytes of a row
-template <> struct Piece<__half> { static constexpr int N = 8; };
-template <> struct Piece<float> { static constexpr int N = 4; };
-
-__device__ __forceinline__ float to_f(__half v) { return __half2float(v); }
-__device__ __forceinline__ float to_f(float v) { return v; }
 __device__ __forceinline__ void from_f(__half& d, float v) { d = __float2half_rn(v); }
 __device__ __forceinline__ void from_f(float& d, float v) { d = v; }
+template <int N>
+__device__ __forceinline__ void add_to(float (&v)[N], const float (&r)[N]) {
+#pragma unroll
+    for (int e = 0; e < N; ++e) v[e] += r[e];
+}
+template <int N>
+__device__ __forceinline__ void add_to(__half (&v)[N], const __half (&r)[N]) {                  // (rounded once)
+#pragma unroll
+    for (int e = 0; e < N; e += 2) {
+        const __half2 s = __hadd2_rn(__halves2half2(v[e], v[e + 1]), __halves2half2(r[e], r[e + 1]));
+        v[e] = __low2half(s);
+        v[e + 1] = __high2half(s);
+    }
+}
+__device__ __forceinline__ float squared_relu(float v) { return v <= 0.f ? 0.f : v * v; }      // (a NaN stays one)
 
-// n valid elements (0..N) at p; VEC: p lies on a 16-byte boundary.
-template <typename T, bool VEC>
-__device__ __forceinline__ void load_piece(const T* p, int n, T (&v)[Piece<T>::N]) {
-    constexpr int N = Piece<T>::N;
-    if (VEC && n == N) {
-        *reinterpret_cast<uint4*>(v) = *reinterpret_cast<const uint4*>(p);
+// U elements (a unit, one access): 16 bytes where rows allow, less where they start on smaller boundaries.
+template <int BYTES> struct Word;
+template <> struct Word<16> { typedef uint4 type; };
+template <> struct Word<8> { typedef uint2 type; };
+template <> struct Word<4> { typedef uint32_t type; };
+template <> struct Word<2> { typedef uint16_t type; };
+template <> struct Word<1> { typedef uint8_t type; };
+template <typename T, int U>
+__device__ __forceinline__ void load_unit(const T* p, int n, T* v) {
+    typedef typename Word<U * (int)sizeof(T)>::type W;
+    if (U == 1 || n >= U) {
+        *reinterpret_cast<W*>(v) = *reinterpret_cast<const W*>(p);
     } else {
 #pragma unroll
-        for (int e = 0; e < N; ++e) {
+        for (int e = 0; e < U; ++e) {
             from_f(v[e], 0.f);
             if (e < n) v[e] = p[e];
         }
     }
 }
-template <typename T, bool VEC>
-__device__ __forceinline__ void store_piece(T* p, int n, const T (&v)[Piece<T>::N]) {
-    constexpr int N = Piece<T>::N;
-    if (VEC && n == N) {
-        *reinterpret_cast<uint4*>(p) = *reinterpret_cast<const uint4*>(v);
+template <typename T, int U>
+__device__ __forceinline__ void store_unit(T* p, int n, const T* v) {
+    typedef typename Word<U * (int)sizeof(T)>::type W;
+    if (U == 1 || n >= U) {
+        *reinterpret_cast<W*>(p) = *reinterpret_cast<const W*>(v);
     } else {
 #pragma unroll
-        for (int e = 0; e < N; ++e)
+        for (int e = 0; e < U; ++e)
             if (e < n) p[e] = v[e];
     }
 }
 
-__device__ __forceinline__ float squared_relu(float v) { return v <= 0.f ? 0.f : v * v; }      // (a NaN stays one)
-
-// TPR threads share a row (32: a warp, eight rows a block; else the block), NP pieces each, which stay in registers.  NP = 0: rows of any
-// length, read again for their codes.
-template <typename T, bool I8, bool VEC, int TPR, int NP>
-__global__ void __launch_bounds__(TPR == 32 ? 256 : TPR) quantize_rows_kernel(const QuantParams p) {
+// TPR threads share a row (32: a warp, eight rows a block; else the block).  A thread holds NP pieces of N elements in registers, a piece being
+// N / U units that neighbouring threads interleave, so that every access of a warp is contiguous.  NP = 0: rows of any length, read again
+// for their codes.
+template <typename T, bool I8, bool RELU2, int U, int TPR, int NP>
+__global__ void __launch_bounds__(TPR == 32 ? 256 : TPR, NP > 0 ? 1536 / (TPR == 32 ? 256 : TPR) : 1) quantize_rows_kernel(const QuantParams p) {
     chain_begin();
-    constexpr int N = Piece<T>::N;
+    constexpr int N = U > 4 ? U : 4, UNITS = N / U;              // elements of a piece, units of it
     constexpr float MOST = I8 ? q8::MOST_I8 : q8::MOST_E4M3;
     const int tid = TPR == 32 ? threadIdx.x & 31 : threadIdx.x, warp = threadIdx.x >> 5;
     const long long row = TPR == 32 ? (long long)blockIdx.x * 8 + warp : (long long)blockIdx.x;
@@ -74,115 +92,128 @@ __global__ void __launch_bounds__(TPR == 32 ? 256 : TPR) quantize_rows_kernel(co
     const T* res = p.residual ? static_cast<const T*>(p.residual) + row * p.ld_res : nullptr;
     T* sum = p.sum ? static_cast<T*>(p.sum) + row * p.ld_sum : nullptr;
     uint8_t* codes = p.codes + row * p.ld_codes;
-    const int pieces = (p.C + N - 1) / N;
-    unsigned top = 0;                                            // max|h| as bits: infinities and NaN order above all numbers
-    float ss = 0.f;
+    float top = 0.f, ss = 0.f;                                   // max|h| (of the numbers; a NaN is in the sum) and sum h^2
+    const auto place = [&](int piece, int unit) { return ((piece * UNITS + unit) * TPR + tid) * U; };
+    const auto has = [&](int piece) { return place(piece, 0) < p.C; };
 
-    auto fetch = [&](int at, T (&v)[N]) {                        // h of piece `at`
-        const int n = min(N, p.C - at * N);
-        load_piece<T, VEC>(x + (long long)at * N, n, v);
-        if (res) {
-            T r[N];
-            load_piece<T, VEC>(res + (long long)at * N, n, r);
+    auto fetch = [&](int piece, T (&v)[N]) {                     // h; zeros behind the row's end
+        T r[N];
 #pragma unroll
-            for (int e = 0; e < N; ++e) from_f(v[e], to_f(v[e]) + to_f(r[e]));
+        for (int u = 0; u < UNITS; ++u) {
+            const int at = place(piece, u);
+#pragma unroll
+            for (int e = 0; e < U; ++e) { from_f(v[u * U + e], 0.f); from_f(r[u * U + e], 0.f); }
+            if (at < p.C) {
+                load_unit<T, U>(x + at, p.C - at, v + u * U);
+                if (res) load_unit<T, U>(res + at, p.C - at, r + u * U);
+            }
+        }
+        if (res) add_to(v, r);
+    };
+    auto values = [&](const T (&v)[N], int e, float (&f)[4]) {
+        q8::four(v + e, f);
+        if constexpr (RELU2) {
+#pragma unroll
+            for (int k = 0; k < 4; ++k) f[k] = squared_relu(f[k]);
         }
     };
     auto look = [&](const T (&v)[N]) {
 #pragma unroll
-        for (int e = 0; e < N; ++e) {
-            const float f = p.relu2 ? squared_relu(to_f(v[e])) : to_f(v[e]);
-            top = max(top, __float_as_uint(f) & 0x7fffffffu);
-            ss = fmaf(f, f, ss);
+        for (int e = 0; e < N; e += 4) {
+            float f[4];
+            values(v, e, f);
+            q8::look_at(top, f);
+#pragma unroll
+            for (int k = 0; k < 4; ++k) ss = fmaf(f[k], f[k], ss);
         }
     };
-    T v[NP ? NP : 1][N];
+    alignas(16) T v[NP ? NP : 1][N];
     if constexpr (NP > 0) {
 #pragma unroll
-        for (int i = 0; i < NP; ++i) {
-            const int at = tid + i * TPR;
-            if (at < pieces) fetch(at, v[i]);
-        }
+        for (int i = 0; i < NP; ++i)
+            if (has(i)) fetch(i, v[i]);
 #pragma unroll
         for (int i = 0; i < NP; ++i)
-            if (tid + i * TPR < pieces) look(v[i]);
+            if (has(i)) look(v[i]);
     } else {
-        for (int at = tid; at < pieces; at += TPR) {
-            fetch(at, v[0]);
+#pragma unroll 1
+        for (int i = 0; has(i); ++i) {
+            fetch(i, v[0]);
             look(v[0]);
         }
     }
 #pragma unroll
     for (int off = 16; off >= 1; off >>= 1) {
-        top = max(top, __shfl_xor_sync(0xffffffffu, top, off));
+        top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, off));
         ss += __shfl_xor_sync(0xffffffffu, ss, off);
     }
     if constexpr (TPR > 32) {
         constexpr int W = TPR / 32;
-        __shared__ unsigned s_top[W];
-        __shared__ float s_ss[W];
+        __shared__ float s_top[W], s_ss[W];
         if ((threadIdx.x & 31) == 0) { s_top[warp] = top; s_ss[warp] = ss; }
         __syncthreads();
         ss = 0.f;
 #pragma unroll
-        for (int w = 0; w < W; ++w) { top = max(top, s_top[w]); ss += s_ss[w]; }
+        for (int w = 0; w < W; ++w) { top = fmaxf(top, s_top[w]); ss += s_ss[w]; }
     }
-    const bool number = top < 0x7f800000u;
-    const float most = __uint_as_float(top);
+    const bool number = top < __uint_as_float(0x7f800000u) && ss == ss, some = number && top > 0.f;
     if (tid == 0) {
-        float s = most;
-        if (p.norm) s = most * (1.0f / sqrtf(ss * p.inv_n + p.eps));
-        p.scale[row] = !number ? __uint_as_float(0x7fc00000u) : top == 0 ? 0.f : s / MOST;
+        float s = top;
+        if (p.norm) s = top * (1.0f / sqrtf(ss * p.inv_n + p.eps));
+        p.scale[row] = !number ? __uint_as_float(0x7fc00000u) : some ? s / MOST : 0.f;
     }
-    const bool some = number && top != 0;
-    const float r = some ? MOST / most : 0.f;
-    const bool wide = !(r < __uint_as_float(0x7f800000u));
-    auto put = [&](int at, const T (&v)[N]) {
-        const int n = min(N, p.C - at * N);
-        if (sum) store_piece<T, VEC>(sum + (long long)at * N, n, v);
+    const q8::Factors factors = q8::factors(MOST, top, q8::den_is_far(top));
+    auto put = [&](int piece, const T (&v)[N]) {
         uint32_t c[N / 4];
 #pragma unroll
         for (int e = 0; e < N; e += 4) {
             float f[4];
-#pragma unroll
-            for (int k = 0; k < 4; ++k) f[k] = p.relu2 ? squared_relu(to_f(v[e + k])) : to_f(v[e + k]);
-            c[e / 4] = some ? q8::codes_of<I8>(f, r, MOST, most, wide) : 0u;
+            values(v, e, f);
+            c[e / 4] = some ? q8::codes_of<I8>(f, factors, MOST, top) : 0u;
         }
-        uint8_t* to = codes + (long long)at * N;
-        if (n == N) {                                            // rows of codes start on 16-byte boundaries
-            if constexpr (N == 8) *reinterpret_cast<uint2*>(to) = make_uint2(c[0], c[1]);
-            else *reinterpret_cast<uint32_t*>(to) = c[0];
-        } else {
 #pragma unroll
-            for (int e = 0; e < N; ++e)
-                if (e < n) to[e] = (uint8_t)(c[e / 4] >> (8 * (e & 3)));
+        for (int u = 0; u < UNITS; ++u) {
+            const int at = place(piece, u);
+            if (at < p.C) {                                      // rows of codes start on 16-byte boundaries
+                if (sum) store_unit<T, U>(sum + at, p.C - at, v + u * U);
+                store_unit<uint8_t, U>(codes + at, p.C - at, reinterpret_cast<const uint8_t*>(c) + u * U);
+            }
         }
     };
     if constexpr (NP > 0) {
 #pragma unroll
-        for (int i = 0; i < NP; ++i) {
-            const int at = tid + i * TPR;
-            if (at < pieces) put(at, v[i]);
-        }
+        for (int i = 0; i < NP; ++i)
+            if (has(i)) put(i, v[i]);
     } else {
-        for (int at = tid; at < pieces; at += TPR) {
-            fetch(at, v[0]);
-            put(at, v[0]);
+#pragma unroll 1
+        for (int i = 0; has(i); ++i) {
+            fetch(i, v[0]);
+            put(i, v[0]);
         }
     }
 }
 
-template <typename T, bool I8, bool VEC>
-int quant_launch(deers_ctx* ctx, const QuantParams& p) {
-    const int pieces = (p.C + Piece<T>::N - 1) / Piece<T>::N;
+template <typename T, bool I8, int U, bool RELU2>
+int quant_widths(deers_ctx* ctx, const QuantParams& p) {
+    constexpr int N = U > 4 ? U : 4;
+    const int pieces = (p.C + N - 1) / N;
     KernelTimerScope ts(ctx, DEERS_K_NORM);
     const unsigned rows = (unsigned)p.rows;
-    if (pieces <= 32) DEERS_CUDA_TRY(ctx, launch_chained(ctx, quantize_rows_kernel<T, I8, VEC, 32, 1>, (rows + 7) / 8, 256, 0, 1, p));
-    else if (pieces <= 128) DEERS_CUDA_TRY(ctx, launch_chained(ctx, quantize_rows_kernel<T, I8, VEC, 32, 4>, (rows + 7) / 8, 256, 0, 1, p));
-    else if (pieces <= 512) DEERS_CUDA_TRY(ctx, launch_chained(ctx, quantize_rows_kernel<T, I8, VEC, 128, 4>, rows, 128, 0, 1, p));
-    else if (pieces <= 2048) DEERS_CUDA_TRY(ctx, launch_chained(ctx, quantize_rows_kernel<T, I8, VEC, 512, 4>, rows, 512, 0, 1, p));
-    else DEERS_CUDA_TRY(ctx, launch_chained(ctx, quantize_rows_kernel<T, I8, VEC, 512, 0>, rows, 512, 0, 1, p));
+#define DEERS_ROWS(TPR, NP) \
+    DEERS_CUDA_TRY(ctx, launch_chained(ctx, quantize_rows_kernel<T, I8, RELU2, U, TPR, NP>, TPR == 32 ? (rows + 7) / 8 : rows, TPR == 32 ? 256 : TPR, 0, 1, p))
+    if (pieces <= 32) DEERS_ROWS(32, 1);
+    else if (pieces <= 64) DEERS_ROWS(32, 2);
+    else if (pieces <= 256) DEERS_ROWS(128, 2);
+    else if (pieces <= 512) DEERS_ROWS(256, 2);
+    else if (pieces <= 1024) DEERS_ROWS(512, 2);
+    else if (pieces <= 2048) DEERS_ROWS(512, 4);
+    else DEERS_ROWS(512, 0);
+#undef DEERS_ROWS
     return DEERS_OK;
+}
+template <typename T, bool I8, int U>
+int quant_launch(deers_ctx* ctx, const QuantParams& p, bool relu2) {
+    return relu2 ? quant_widths<T, I8, U, true>(ctx, p) : quant_widths<T, I8, U, false>(ctx, p);
 }
 
 }  // namespace
@@ -206,15 +237,14 @@ extern "C" int deers_b200_quantize_rows(deers_ctx* ctx, const deers_quantize_des
     p.x = x; p.residual = residual; p.sum = sum; p.codes = (uint8_t*)codes; p.scale = scale;
     p.ld_x = d->ld_x; p.ld_res = residual ? d->ld_residual : 0; p.ld_sum = sum ? d->ld_sum : 0; p.ld_codes = d->ld_codes;
     p.rows = d->rows; p.C = d->C; p.eps = (float)d->eps; p.inv_n = (float)(1.0 / (double)d->C);
-    p.norm = d->norm; p.relu2 = d->relu_squared;
-    const bool vec = (((uintptr_t)x | (uintptr_t)residual | (uintptr_t)sum) & 15u) == 0 &&
-                     ((p.ld_x | p.ld_res | p.ld_sum) * (long long)es & 15) == 0;
-    const bool half = d->dtype == DEERS_F16, i8 = d->code == DEERS_I8;
-    const auto go = half ? (i8 ? (vec ? quant_launch<__half, true, true> : quant_launch<__half, true, false>)
-                               : (vec ? quant_launch<__half, false, true> : quant_launch<__half, false, false>))
-                         : (i8 ? (vec ? quant_launch<float, true, true> : quant_launch<float, true, false>)
-                               : (vec ? quant_launch<float, false, true> : quant_launch<float, false, false>));
-    const int rc = go(ctx, p);
+    p.norm = d->norm;
+    const uintptr_t at = (uintptr_t)x | (uintptr_t)residual | (uintptr_t)sum | (uintptr_t)((p.ld_x | p.ld_res | p.ld_sum) * (long long)es);
+    const bool half = d->dtype == DEERS_F16, i8 = d->code == DEERS_I8, wide = (at & 15) == 0, half16 = (at & 7) == 0, pair = (at & 3) == 0;
+    const auto go = half ? (i8 ? (wide ? quant_launch<__half, true, 8> : half16 ? quant_launch<__half, true, 4> : pair ? quant_launch<__half, true, 2> : quant_launch<__half, true, 1>)
+                               : (wide ? quant_launch<__half, false, 8> : half16 ? quant_launch<__half, false, 4> : pair ? quant_launch<__half, false, 2> : quant_launch<__half, false, 1>))
+                         : (i8 ? (wide ? quant_launch<float, true, 4> : half16 ? quant_launch<float, true, 2> : quant_launch<float, true, 1>)
+                               : (wide ? quant_launch<float, false, 4> : half16 ? quant_launch<float, false, 2> : quant_launch<float, false, 1>));
+    const int rc = go(ctx, p, d->relu_squared != 0);
     if (rc) return rc;
     ctx->launches += 1;
     DEERS_CUDA_TRY(ctx, cudaGetLastError());
