@@ -7,8 +7,8 @@
 // has half the time per value that an f16 cache leaves: by f32 instructions alone a value costs a conversion and a multiplication for
 // every query row, by these products 0.5 to 0.75 conversion instructions and a 32nd of two products whatever R is up to eight.
 //
-//   A warp takes blocks of 32 keys (one scale each) in turn.  Every lane copies (cp.async) the bytes that its own fragments need into a ring in
-//   shared memory and reads back only what it wrote: no barrier in the walk, several blocks in flight, no registers held by them.
+//   A warp takes blocks of 32 keys (one scale each) in turn, which TMA brings into a ring of its own in shared memory (swizzled, so that lanes read
+//   without conflicts, or two by two): a block costs one lane two copies, and warps wait for nobody but their own.
 //   S^T = K Q^T: the order of the channels inside a product is free as long as K and Q agree, so a lane's 16 consecutive bytes of a key
 //   are its share of four products.  O^T += V^T P^T: the order of the keys is free too, and a lane's bytes of two keys are interleaved by
 //   byte permutations, which is the transposition that V needs.  P moves from the first product's layout to the second's by movmatrix.
@@ -21,6 +21,8 @@
 
 #include "common.cuh"
 #include "q8_codes.cuh"
+#include "sm100_ptx.cuh"
+#include "tma_host.cuh"
 
 #include <cooperative_groups.h>
 
@@ -59,15 +61,6 @@ __device__ __forceinline__ uint32_t transposed(uint32_t a) {
     asm volatile("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(d) : "r"(a));
     return d;
 }
-template <int BYTES>
-__device__ __forceinline__ void copy_in(uint32_t dst, const uint8_t* src, uint32_t n) {
-    if constexpr (BYTES == 16) asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(n) : "memory");
-    else asm volatile("cp.async.ca.shared.global [%0], [%1], 8, %2;" ::"r"(dst), "l"(src), "r"(n) : "memory");
-}
-__device__ __forceinline__ void copies_end_group() { asm volatile("cp.async.commit_group;" ::: "memory"); }
-template <int N>
-__device__ __forceinline__ void copies_wait() { asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory"); }
-
 // 2^x for x <= 0 (results below 2^-126 are zero).
 __device__ __forceinline__ float power2(float x) {
     float y;
@@ -85,24 +78,43 @@ struct Shape {
     static constexpr int VB = DP >= 128 ? 16 : 8;                // bytes of a piece of V: at VB * (lane / 4 + 8 c)
     static constexpr int VC = DP / 8 / VB;
     static constexpr int STAGES = DP == 64 ? 4 : 2;
-    static constexpr int STAGE_BYTES = 32 * 2 * DP;              // 32 keys: every byte of them is some lane's
+    static constexpr int STAGE_BYTES = 32 * 2 * DP;              // 32 keys, K and V
+    static constexpr int BOX = DP == 64 ? 64 : 128, BOXES = DP / BOX;     // bytes of a key in a box of 32 keys, boxes of K or of V
     static constexpr int RING = DQ_WARPS * STAGES * STAGE_BYTES;
     static constexpr int ROWS = 8 * NT;
     static constexpr int OS = DP + 4;                            // row of partial results: O, then maximum and sum
     static constexpr int MERGE = DQ_WARPS * ROWS * OS * 4;
     static constexpr int PART = ROWS * OS * 4;
-    static constexpr int SMEM = RING > MERGE + PART ? RING : MERGE + PART;         // (the ring has been read when the warps meet)
+    static constexpr int BARS = RING > MERGE + PART ? RING : MERGE + PART;         // (the ring has been read when the warps meet)
+    static constexpr int SMEM = BARS + DQ_WARPS * STAGES * 8 + 16;
 };
 
 enum DecodeQ8End { DQ_ONE_CHUNK = 0, DQ_CLUSTER = 1, DQ_TO_WORKSPACE = 2 };
 
+// Barriers: nothing of global memory.
+template <int DP, int NT>
+__device__ __forceinline__ void decode_q8_prologue(const void* tmap_k, const void* tmap_v) {
+    using S = Shape<DP, NT>;
+    extern __shared__ __align__(1024) uint8_t smem[];
+    uint64_t* bars = reinterpret_cast<uint64_t*>(smem + S::BARS);
+    uint32_t* abort_s = reinterpret_cast<uint32_t*>(bars + DQ_WARPS * S::STAGES);
+    if (threadIdx.x == 0) {
+        for (int i = 0; i < DQ_WARPS * S::STAGES; ++i) sm100::mbar_init(&bars[i], 1);
+        abort_s[0] = 0;
+        sm100::fence_barrier_init();
+        sm100::tma_prefetch_desc(tmap_k); sm100::tma_prefetch_desc(tmap_v);
+    }
+}
+
 template <typename T, int DP, int NT, int END>
-__global__ void __launch_bounds__(32 * DQ_WARPS) decode_q8_kernel(const DecodeQ8Params p) {
+__global__ void __launch_bounds__(32 * DQ_WARPS)
+decode_q8_kernel(const __grid_constant__ CUtensorMap tmap_k, const __grid_constant__ CUtensorMap tmap_v, const DecodeQ8Params p) {
+    decode_q8_prologue<DP, NT>(&tmap_k, &tmap_v);
     chain_wait();
     using S = Shape<DP, NT>;
     constexpr bool F32 = sizeof(T) == 4;
     constexpr int QP = F32 ? 2 : 1;                              // f16 parts of a value of q
-    extern __shared__ __align__(16) uint8_t smem[];
+    extern __shared__ __align__(1024) uint8_t smem[];
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
     const int split = blockIdx.x, Hkv = p.H / p.G, b = blockIdx.y / Hkv, kvh = blockIdx.y % Hkv, tile = blockIdx.z;
     const int R = p.G * p.Tq, row0 = tile * S::ROWS;
@@ -114,62 +126,33 @@ __global__ void __launch_bounds__(32 * DQ_WARPS) decode_q8_kernel(const DecodeQ8
     // this block's keys: its share of the sequence's blocks of 32
     const int blocks = (len + 31) / 32;
     const int blk0 = (int)((long long)blocks * split / p.splits), blk1 = (int)((long long)blocks * (split + 1) / p.splits);
-    const uint8_t* kb = p.k + b * p.sk[0] + kvh * p.sk[1];
     const uint8_t* vb = p.v + b * p.sv[0] + kvh * p.sv[1];
     const float* ksl = p.k_scale + b * p.skl[0] + kvh * p.skl[1];
     const float* vsl = p.v_scale + b * p.svl[0] + kvh * p.svl[1];
 
+    __syncthreads();                                             // the barriers are there
     uint8_t* ring = smem + warp * (S::STAGES * S::STAGE_BYTES);
-    const uint32_t ring_u = (uint32_t)__cvta_generic_to_shared(ring) + lane * 16;
-    const uint32_t vring_u = (uint32_t)__cvta_generic_to_shared(ring) + 32 * DP + lane * S::VB;
-    // This lane's keys of a block: 8 r + g of K; 2t, 2t + 1, 2t + 8, 2t + 9 of either half of V.
-    const auto k_key = [&](int r) { return 8 * r + g; };
-    const auto v_key = [&](int r) { return (r >> 2) * 16 + ((r >> 1) & 1) * 8 + 2 * t + (r & 1); };
-    uint32_t k_at[4], v_at[8], k_size[S::KC], v_size[S::VC];     // their places relative to the block's, and the bytes that a piece has
-#pragma unroll
-    for (int r = 0; r < 4; ++r) k_at[r] = (uint32_t)k_key(r) * (uint32_t)p.sk[2] + 16 * t;
-#pragma unroll
-    for (int r = 0; r < 8; ++r) v_at[r] = (uint32_t)v_key(r) * (uint32_t)p.sv[2] + S::VB * g;
-#pragma unroll
-    for (int c = 0; c < S::KC; ++c) k_size[c] = 16 * (t + 4 * c) < p.D ? 16 : 0;
-#pragma unroll
-    for (int c = 0; c < S::VC; ++c) v_size[c] = S::VB * (g + 8 * c) < p.D ? S::VB : 0;
-    // Fetches block `blk` into stage s.  Keys behind the last are zeros: what lies there belongs to nobody.
+    uint64_t* full = reinterpret_cast<uint64_t*>(smem + S::BARS) + warp * S::STAGES;
+    const sm100::WaitState ws{reinterpret_cast<uint32_t*>(smem + S::BARS + DQ_WARPS * S::STAGES * 8), p.err};
+    // Block `blk` into stage s, by one lane.  (Keys behind the sequence's last may lie in it, and are masked below.)
     auto fetch = [&](int blk, int s) {
-        if (blk < blk1) {
-            const uint8_t* kp = kb + (long long)blk * 32 * p.sk[2];
-            const uint8_t* vp = vb + (long long)blk * 32 * p.sv[2];
-            const int left = len - blk * 32;                     // keys from here on
-            if (left >= 32) {
+        if (blk < blk1 && lane == 0) {
+            sm100::mbar_arrive_expect_tx(&full[s], S::STAGE_BYTES);
 #pragma unroll
-                for (int r = 0; r < 4; ++r)
-#pragma unroll
-                    for (int c = 0; c < S::KC; ++c)
-                        copy_in<16>(ring_u + s * S::STAGE_BYTES + (r * S::KC + c) * 512, kp + k_at[r] + (DP > 64 && k_size[c] ? 64 * c : 0), k_size[c]);
-#pragma unroll
-                for (int r = 0; r < 8; ++r)
-#pragma unroll
-                    for (int c = 0; c < S::VC; ++c)
-                        copy_in<S::VB>(vring_u + s * S::STAGE_BYTES + (r * S::VC + c) * (32 * S::VB), vp + v_at[r] + (S::VC > 1 && v_size[c] ? 128 * c : 0), v_size[c]);
-            } else {
-#pragma unroll
-                for (int r = 0; r < 4; ++r)
-#pragma unroll
-                    for (int c = 0; c < S::KC; ++c) {
-                        const uint32_t n = k_key(r) < left ? k_size[c] : 0;
-                        copy_in<16>(ring_u + s * S::STAGE_BYTES + (r * S::KC + c) * 512, n ? kp + k_at[r] + 64 * c : kb, n);
-                    }
-#pragma unroll
-                for (int r = 0; r < 8; ++r)
-#pragma unroll
-                    for (int c = 0; c < S::VC; ++c) {
-                        const uint32_t n = v_key(r) < left ? v_size[c] : 0;
-                        copy_in<S::VB>(vring_u + s * S::STAGE_BYTES + (r * S::VC + c) * (32 * S::VB), n ? vp + v_at[r] + 128 * c : vb, n);
-                    }
+            for (int i = 0; i < S::BOXES; ++i) {
+                sm100::tma_load_4d(ring + s * S::STAGE_BYTES + i * 32 * S::BOX, &tmap_k, &full[s], i * S::BOX, blk * 32, kvh, b);
+                sm100::tma_load_4d(ring + s * S::STAGE_BYTES + 32 * DP + i * 32 * S::BOX, &tmap_v, &full[s], i * S::BOX, blk * 32, kvh, b);
             }
         }
-        copies_end_group();
     };
+    // 16 bytes of key j at 16 * piece (bytes 8 * half of them) inside the boxes of K or of V
+    auto in_boxes = [&](int j, int piece) {
+        if constexpr (DP == 64) return j * 64 + ((piece ^ (j >> 1 & 3)) << 4);
+        else return (piece >> 3) * (32 * 128) + j * 128 + (((piece & 7) ^ (j & 7)) << 4);
+    };
+    // This lane's keys of a block: 8 r + g of K; 2t, 2t + 1, 2t + 8, 2t + 9 of either half of V.
+    const auto v_key = [&](int r) { return (r >> 2) * 16 + ((r >> 1) & 1) * 8 + 2 * t + (r & 1); };
+    const auto v_at = [&](int r, int c) { return 32 * DP + (DP == 64 ? in_boxes(v_key(r), g >> 1) + 8 * (g & 1) : in_boxes(v_key(r), g + 8 * c)); };
 #pragma unroll
     for (int s = 0; s < S::STAGES - 1; ++s) fetch(blk0 + warp + s * DQ_WARPS, s);
 
@@ -252,17 +235,16 @@ __global__ void __launch_bounds__(32 * DQ_WARPS) decode_q8_kernel(const DecodeQ8
     }
 
     int stage = 0;
+    uint32_t phase = 0;
     float ks_next = 0.f, vs_next = 0.f;                          // scales of the next round's block
     if (blk0 + warp < blk1) { ks_next = ksl[blk0 + warp]; vs_next = vsl[blk0 + warp]; }
 #pragma unroll 1
     for (int blk = blk0 + warp; blk < blk1; blk += DQ_WARPS) {
         const float ks = ks_next, vs = vs_next;
         if (blk + DQ_WARPS < blk1) { ks_next = ksl[blk + DQ_WARPS]; vs_next = vsl[blk + DQ_WARPS]; }
-        copies_wait<S::STAGES - 2>();
-        {
-            const int into = stage == 0 ? S::STAGES - 1 : stage - 1;         // the stage that the last round has read
-            fetch(blk + (S::STAGES - 1) * DQ_WARPS, into);
-        }
+        __syncwarp();
+        fetch(blk + (S::STAGES - 1) * DQ_WARPS, stage == 0 ? S::STAGES - 1 : stage - 1);      // (the stage that the last round has read)
+        if (!sm100::mbar_wait_warp(ws, &full[stage], phase, DEERS_KERR_CACHE | 3u)) break;
         const uint8_t* st = ring + stage * S::STAGE_BYTES;
         // ---- scores: keys 16 mt + g and 16 mt + g + 8.  The tensor core cuts its sums off, towards zero: with f32 queries the chains are short (a
         // piece of a key each, the low parts of q apart) and added in f32.
@@ -279,8 +261,8 @@ __global__ void __launch_bounds__(32 * DQ_WARPS) decode_q8_kernel(const DecodeQ8
                     for (int e = 0; e < 4; ++e) sum[nt][i][e] = 0.f;
 #pragma unroll
             for (int c = 0; c < S::KC; ++c) {
-                const uint4 x = *reinterpret_cast<const uint4*>(st + ((2 * mt) * S::KC + c) * 512 + lane * 16);
-                const uint4 y = *reinterpret_cast<const uint4*>(st + ((2 * mt + 1) * S::KC + c) * 512 + lane * 16);
+                const uint4 x = *reinterpret_cast<const uint4*>(st + in_boxes(16 * mt + g, t + 4 * c));
+                const uint4 y = *reinterpret_cast<const uint4*>(st + in_boxes(16 * mt + 8 + g, t + 4 * c));
                 const uint32_t xw[4] = {x.x, x.y, x.z, x.w}, yw[4] = {y.x, y.y, y.z, y.w};
 #pragma unroll
                 for (int w = 0; w < 4; ++w) {
@@ -372,11 +354,14 @@ __global__ void __launch_bounds__(32 * DQ_WARPS) decode_q8_kernel(const DecodeQ8
         if (edge && lim_min < len) {
             uint32_t nan = 0;
 #pragma unroll
-            for (int r = 0; r < 8 * S::VC; ++r) {
-                const uint8_t* src = st + 32 * DP + r * (32 * S::VB) + lane * S::VB;
+            for (int r = 0; r < 8; ++r)
 #pragma unroll
-                for (int w = 0; w < S::VB / 4; ++w) nan |= ((reinterpret_cast<const uint32_t*>(src)[w] & 0x7f7f7f7fu) + 0x01010101u) & 0x80808080u;
-            }
+                for (int c = 0; c < S::VC; ++c) {
+                    if (v_key(r) >= len - blk * 32) continue;
+#pragma unroll
+                    for (int w = 0; w < S::VB / 4; ++w)
+                        nan |= ((reinterpret_cast<const uint32_t*>(st + v_at(r, c))[w] & 0x7f7f7f7fu) + 0x01010101u) & 0x80808080u;
+                }
             if (__any_sync(0xffffffffu, nan != 0)) {
                 if constexpr (F32) {
 #pragma unroll
@@ -410,7 +395,7 @@ __global__ void __launch_bounds__(32 * DQ_WARPS) decode_q8_kernel(const DecodeQ8
                                 }
                             }
                         }
-                stage = stage + 1 == S::STAGES ? 0 : stage + 1;
+                if (++stage == S::STAGES) { stage = 0; phase ^= 1u; }
                 continue;
             }
         }
@@ -423,10 +408,20 @@ __global__ void __launch_bounds__(32 * DQ_WARPS) decode_q8_kernel(const DecodeQ8
             for (int mt = 0; mt < 2; ++mt)
 #pragma unroll
                 for (int r = 0; r < 4; ++r) {
-                    const uint8_t* src = st + 32 * DP + ((4 * mt + r) * S::VC + c) * (32 * S::VB) + lane * S::VB;
+                    const uint8_t* src = st + v_at(4 * mt + r, c);
                     if constexpr (VW == 4) *reinterpret_cast<uint4*>(x[mt][r]) = *reinterpret_cast<const uint4*>(src);
                     else *reinterpret_cast<uint2*>(x[mt][r]) = *reinterpret_cast<const uint2*>(src);
                 }
+            if (blk * 32 + 32 > len) {                           // what lies behind the last key is nobody's, and may be NaN
+#pragma unroll
+                for (int mt = 0; mt < 2; ++mt)
+#pragma unroll
+                    for (int r = 0; r < 4; ++r)
+                        if (v_key(4 * mt + r) >= len - blk * 32) {
+#pragma unroll
+                            for (int w = 0; w < VW; ++w) x[mt][r][w] = 0;
+                        }
+            }
 #pragma unroll
             for (int w = 0; w < VW; ++w)
 #pragma unroll
@@ -457,9 +452,8 @@ __global__ void __launch_bounds__(32 * DQ_WARPS) decode_q8_kernel(const DecodeQ8
                     }
                 }
         }
-        stage = stage + 1 == S::STAGES ? 0 : stage + 1;
+        if (++stage == S::STAGES) { stage = 0; phase ^= 1u; }
     }
-    copies_wait<0>();
     chain_next();
 
     // ---- the warps meet
@@ -642,6 +636,9 @@ int decode_q8_check(const deers_decode_q8_desc* d) {
     if (!(d->scale == d->scale)) return DEERS_ERR_SHAPE;
     if (d->Tq > 128 || d->Tq > d->cache.capacity || (long long)d->cache.B * d->cache.H > 65535 || (long long)d->H / d->cache.H * d->Tq > 65535)
         return DEERS_ERR_UNSUPPORTED;
+    // (maps of the copies want strides that advance)
+    if (d->cache.B > 1 && (d->cache.k_strides[0] == 0 || d->cache.v_strides[0] == 0)) return DEERS_ERR_LAYOUT;
+    if (d->cache.H > 1 && (d->cache.k_strides[1] == 0 || d->cache.v_strides[1] == 0)) return DEERS_ERR_LAYOUT;
     for (const int64_t* s : {d->q_strides, d->o_strides}) {
         if (s[3] != 1) return DEERS_ERR_LAYOUT;
         for (int i = 0; i < 3; ++i)
@@ -650,19 +647,33 @@ int decode_q8_check(const deers_decode_q8_desc* d) {
     return DEERS_OK;
 }
 
+// Map over the codes of a cache, [D, capacity, H, B] (innermost first): boxes of 32 keys, zeros outside.
+int tmap_cache(deers_ctx* ctx, CUtensorMap* out, const void* base, const deers_cache_q8& c, const int64_t* st, int box) {
+    const cuuint64_t dims[4] = {(cuuint64_t)c.D, (cuuint64_t)c.capacity, (cuuint64_t)c.H, (cuuint64_t)c.B};
+    // (an axis of one place never advances: any legal stride)
+    const cuuint64_t t = (cuuint64_t)st[2], h = c.H > 1 ? (cuuint64_t)st[1] : t * dims[1], b = c.B > 1 ? (cuuint64_t)st[0] : h * dims[2];
+    const cuuint64_t strides[3] = {t, h, b};
+    const cuuint32_t boxes[4] = {(cuuint32_t)box, 32, 1, 1};
+    return make_tmap_bytes(ctx, out, base, dims, strides, boxes, box == 64 ? CU_TENSOR_MAP_SWIZZLE_64B : CU_TENSOR_MAP_SWIZZLE_128B);
+}
+
 template <typename T, int DP, int NT>
-int decode_q8_launch(deers_ctx* ctx, const DecodeQ8Params& p, const DecodeQ8Plan& plan, int slices) {
+int decode_q8_launch(deers_ctx* ctx, const DecodeQ8Params& p, const DecodeQ8Plan& plan, int slices, const deers_cache_q8& cache) {
     using S = Shape<DP, NT>;
+    CUtensorMap tk, tv;
+    int rc = tmap_cache(ctx, &tk, cache.k, cache, cache.k_strides, S::BOX);
+    if (!rc) rc = tmap_cache(ctx, &tv, cache.v, cache, cache.v_strides, S::BOX);
+    if (rc) return rc;
     const dim3 grid(plan.splits, slices, plan.tiles);
     if (plan.end == DQ_ONE_CHUNK) {
         DEERS_SMEM_ONCE(ctx, (decode_q8_kernel<T, DP, NT, DQ_ONE_CHUNK>), S::SMEM);
-        DEERS_CUDA_TRY(ctx, launch_chained(ctx, decode_q8_kernel<T, DP, NT, DQ_ONE_CHUNK>, grid, 32 * DQ_WARPS, S::SMEM, 1, p));
+        DEERS_CUDA_TRY(ctx, launch_chained(ctx, decode_q8_kernel<T, DP, NT, DQ_ONE_CHUNK>, grid, 32 * DQ_WARPS, S::SMEM, 1, tk, tv, p));
     } else if (plan.end == DQ_CLUSTER) {
         DEERS_SMEM_ONCE(ctx, (decode_q8_kernel<T, DP, NT, DQ_CLUSTER>), S::SMEM);
-        DEERS_CUDA_TRY(ctx, launch_chained(ctx, decode_q8_kernel<T, DP, NT, DQ_CLUSTER>, grid, 32 * DQ_WARPS, S::SMEM, plan.splits, p));
+        DEERS_CUDA_TRY(ctx, launch_chained(ctx, decode_q8_kernel<T, DP, NT, DQ_CLUSTER>, grid, 32 * DQ_WARPS, S::SMEM, plan.splits, tk, tv, p));
     } else {
         DEERS_SMEM_ONCE(ctx, (decode_q8_kernel<T, DP, NT, DQ_TO_WORKSPACE>), S::SMEM);
-        DEERS_CUDA_TRY(ctx, launch_chained(ctx, decode_q8_kernel<T, DP, NT, DQ_TO_WORKSPACE>, grid, 32 * DQ_WARPS, S::SMEM, 1, p));
+        DEERS_CUDA_TRY(ctx, launch_chained(ctx, decode_q8_kernel<T, DP, NT, DQ_TO_WORKSPACE>, grid, 32 * DQ_WARPS, S::SMEM, 1, tk, tv, p));
         const dim3 rows(S::ROWS, slices, plan.tiles);
         DEERS_CUDA_TRY(ctx, launch_chained(ctx, decode_q8_join_kernel<T>, rows, 128, 0, 1, p, S::ROWS, plan.tiles));
         ctx->launches += 1;
@@ -671,10 +682,10 @@ int decode_q8_launch(deers_ctx* ctx, const DecodeQ8Params& p, const DecodeQ8Plan
 }
 
 template <typename T>
-int decode_q8_widths(deers_ctx* ctx, const DecodeQ8Params& p, const DecodeQ8Plan& plan, int slices) {
-    if (plan.dp == 64) return plan.nt == 2 ? decode_q8_launch<T, 64, 2>(ctx, p, plan, slices) : decode_q8_launch<T, 64, 1>(ctx, p, plan, slices);
-    if (plan.dp == 128) return plan.nt == 2 ? decode_q8_launch<T, 128, 2>(ctx, p, plan, slices) : decode_q8_launch<T, 128, 1>(ctx, p, plan, slices);
-    return decode_q8_launch<T, 256, 1>(ctx, p, plan, slices);
+int decode_q8_widths(deers_ctx* ctx, const DecodeQ8Params& p, const DecodeQ8Plan& plan, int slices, const deers_cache_q8& c) {
+    if (plan.dp == 64) return plan.nt == 2 ? decode_q8_launch<T, 64, 2>(ctx, p, plan, slices, c) : decode_q8_launch<T, 64, 1>(ctx, p, plan, slices, c);
+    if (plan.dp == 128) return plan.nt == 2 ? decode_q8_launch<T, 128, 2>(ctx, p, plan, slices, c) : decode_q8_launch<T, 128, 1>(ctx, p, plan, slices, c);
+    return decode_q8_launch<T, 256, 1>(ctx, p, plan, slices, c);
 }
 
 }  // namespace
@@ -707,7 +718,7 @@ extern "C" int deers_b200_attn_decode_q8(deers_ctx* ctx, const deers_decode_q8_d
     p.q_vec = ((uintptr_t)q & 15u) == 0 && ((d->q_strides[0] | d->q_strides[1] | d->q_strides[2]) & al) == 0;
     {
         KernelTimerScope ts(ctx, DEERS_K_DECODE);
-        rc = d->dtype == DEERS_F16 ? decode_q8_widths<__half>(ctx, p, plan, c.B * c.H) : decode_q8_widths<float>(ctx, p, plan, c.B * c.H);
+        rc = d->dtype == DEERS_F16 ? decode_q8_widths<__half>(ctx, p, plan, c.B * c.H, c) : decode_q8_widths<float>(ctx, p, plan, c.B * c.H, c);
         if (rc) return rc;
     }
     ctx->launches += 1;

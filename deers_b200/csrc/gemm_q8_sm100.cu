@@ -9,7 +9,7 @@
 // What bounds them: large ones the tensor pipe; steps the weight's bytes (here 8 us) and, before and behind them, 2 us to the first K block and 2 to 4 from the
 // last product to the end.
 #include "sm100_ptx.cuh"
-#include "common.cuh"
+#include "tma_host.cuh"
 
 #include <cooperative_groups.h>
 
@@ -462,27 +462,11 @@ gemm_q8_split_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid_co
     if (warp == 1) tmem_dealloc(tmem, S::TMEM);
 }
 
-typedef CUresult (*EncodeTiled)(CUtensorMap*, CUtensorMapDataType, cuuint32_t, void*, const cuuint64_t*, const cuuint64_t*, const cuuint32_t*,
-                                const cuuint32_t*, CUtensorMapInterleave, CUtensorMapSwizzle, CUtensorMapL2promotion, CUtensorMapFloatOOBfill);
-
 // Map over [rows][inner] bytes, rows ld bytes apart: boxes of 128 bytes by box_rows rows, 128-byte swizzle, zeros outside.
 int tmap_bytes(deers_ctx* ctx, CUtensorMap* out, const void* base, long long rows, long long inner, long long ld, int box_rows) {
-    if (!ctx->encode_tiled) {
-        snprintf(ctx->last_error, sizeof(ctx->last_error), "cuTensorMapEncodeTiled not available");
-        return DEERS_ERR_CUDA;
-    }
-    const cuuint64_t dims[4] = {(cuuint64_t)inner, (cuuint64_t)rows, 1, 1};
-    const cuuint64_t far = (cuuint64_t)ld * (cuuint64_t)rows;
-    const cuuint64_t strides[3] = {(cuuint64_t)ld, far, far};
-    const cuuint32_t box[4] = {(cuuint32_t)QK, (cuuint32_t)box_rows, 1, 1}, one[4] = {1, 1, 1, 1};
-    const CUresult r = ((EncodeTiled)ctx->encode_tiled)(out, CU_TENSOR_MAP_DATA_TYPE_UINT8, 4, const_cast<void*>(base), dims, strides, box, one,
-                                                        CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B,
-                                                        CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
-    if (r != CUDA_SUCCESS) {
-        snprintf(ctx->last_error, sizeof(ctx->last_error), "cuTensorMapEncodeTiled failed with CUresult %d", (int)r);
-        return DEERS_ERR_LAYOUT;
-    }
-    return DEERS_OK;
+    const cuuint64_t dims[4] = {(cuuint64_t)inner, (cuuint64_t)rows, 1, 1}, far = (cuuint64_t)ld * (cuuint64_t)rows, strides[3] = {(cuuint64_t)ld, far, far};
+    const cuuint32_t box[4] = {(cuuint32_t)QK, (cuuint32_t)box_rows, 1, 1};
+    return make_tmap_bytes(ctx, out, base, dims, strides, box, CU_TENSOR_MAP_SWIZZLE_128B);
 }
 
 struct GemmQ8Plan { int bn, parts; bool swap, split, pair; };

@@ -35,3 +35,21 @@ static inline int make_tmap_bhtd_f16(deers_ctx* ctx, CUtensorMap* out, const voi
     }
     return DEERS_OK;
 }
+
+// Tensor map over bytes, four dimensions (innermost first, strides of the outer three in bytes), out-of-range bytes read as zero.
+static inline int make_tmap_bytes(deers_ctx* ctx, CUtensorMap* out, const void* base, const cuuint64_t* dims, const cuuint64_t* strides,
+                                  const cuuint32_t* box, CUtensorMapSwizzle swizzle) {
+    if (!ctx->encode_tiled) {
+        snprintf(ctx->last_error, sizeof(ctx->last_error), "cuTensorMapEncodeTiled not available");
+        return DEERS_ERR_CUDA;
+    }
+    const cuuint32_t one[4] = {1u, 1u, 1u, 1u};
+    const CUresult r = ((PFN_encodeTiled)ctx->encode_tiled)(
+        out, CU_TENSOR_MAP_DATA_TYPE_UINT8, 4, const_cast<void*>(base), dims, strides, box, one, CU_TENSOR_MAP_INTERLEAVE_NONE, swizzle,
+        CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+    if (r != CUDA_SUCCESS) {
+        snprintf(ctx->last_error, sizeof(ctx->last_error), "cuTensorMapEncodeTiled failed with CUresult %d", (int)r);
+        return DEERS_ERR_LAYOUT;
+    }
+    return DEERS_OK;
+}
