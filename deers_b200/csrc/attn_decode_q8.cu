@@ -25,13 +25,14 @@
 #include "tma_host.cuh"
 
 #include <cooperative_groups.h>
+#include <stdlib.h>
 
 int deers_check_cache(const deers_cache_q8* c);
 
 namespace {
 
 constexpr int DQ_WARPS = 4;
-constexpr int DQ_MAX_SPLITS = 4 * 148;
+constexpr int DQ_MAX_BLOCKS = 3 * 148, DQ_MAX_EVEN = 256;        // blocks of threads and sequences of an even share
 constexpr float DQ_LOG2E = 1.4426950408889634f, DQ_LN2 = 0.6931471805599453f;
 constexpr float DQ_UP = 32768.0f;                                // weights are at most 2^15 of f16's 65504
 
@@ -39,9 +40,10 @@ struct DecodeQ8Params {
     const void* q; void* o; float* lse;
     const uint8_t* k; const uint8_t* v; const float* k_scale; const float* v_scale;
     const int* lengths;
-    float* part;                                                 // [slice][tile][split][rows of a tile][D + 2]
+    long long* before;                                           // DQ_EVEN: [B + 1] blocks of all slices of the sequences before
+    float* part;                                                 // [block of threads][2][rows of a tile][D + 4]: O, maximum, sum
     long long sq[3], so[3], sk[3], sv[3], skl[2], svl[2];
-    int H, G, Tq, D, cap, causal, splits, q_vec;
+    int B, H, G, Tq, D, cap, causal, splits, tiles, q_vec, o_vec;
     float scale;
     unsigned int* err;
 };
@@ -68,8 +70,24 @@ __device__ __forceinline__ float power2(float x) {
     return y;
 }
 
+__device__ __forceinline__ void add4(float4& v, float w, const float4& x) {
+    v.x = fmaf(w, x.x, v.x); v.y = fmaf(w, x.y, v.y); v.z = fmaf(w, x.z, v.z); v.w = fmaf(w, x.w, v.w);
+}
+__device__ __forceinline__ void send4(uint32_t to, const float4& v) {
+    asm volatile("st.shared::cluster.v4.f32 [%0], {%1, %2, %3, %4};" ::"r"(to), "f"(v.x), "f"(v.y), "f"(v.z), "f"(v.w) : "memory");
+}
+__device__ __forceinline__ void send(uint32_t to, float v) { asm volatile("st.shared::cluster.f32 [%0], %1;" ::"r"(to), "f"(v) : "memory"); }
 __device__ __forceinline__ void put(float* p, float v) { *p = v; }
 __device__ __forceinline__ void put(__half* p, float v) { *p = __float2half_rn(v); }
+// Four channels; vec: rows of o lie on 16-byte boundaries.
+__device__ __forceinline__ void put4(float* p, const float4& v, int vec) {
+    if (vec) *reinterpret_cast<float4*>(p) = v;
+    else { p[0] = v.x; p[1] = v.y; p[2] = v.z; p[3] = v.w; }
+}
+__device__ __forceinline__ void put4(__half* p, const float4& v, int vec) {
+    if (vec) *reinterpret_cast<uint2*>(p) = make_uint2(pack2(v.x, v.y), pack2(v.z, v.w));
+    else { put(p, v.x); put(p + 1, v.y); put(p + 2, v.z); put(p + 3, v.w); }
+}
 
 // Shapes of a kernel for heads of up to DP channels and 8 * NT query rows.
 template <int DP, int NT>
@@ -84,12 +102,23 @@ struct Shape {
     static constexpr int ROWS = 8 * NT;
     static constexpr int OS = DP + 4;                            // row of partial results: O, then maximum and sum
     static constexpr int MERGE = DQ_WARPS * ROWS * OS * 4;
-    static constexpr int PART = ROWS * OS * 4;
-    static constexpr int BARS = RING > MERGE + PART ? RING : MERGE + PART;         // (the ring has been read when the warps meet)
-    static constexpr int SMEM = BARS + DQ_WARPS * STAGES * 8 + 16;
+    static constexpr int PART = ROWS * DP * 4;                   // DQ_CLUSTER: [block][its share of O] and, before, [block][row] maximum and sum
+    // (the ring has been read when the warps meet; what other blocks of a cluster send has a place of its own)
+    static constexpr int SENT = RING > MERGE ? RING : MERGE, BARS = SENT + 8 * ROWS * 8 + PART + 8 * 32;
+    static constexpr int SMEM = BARS + DQ_WARPS * STAGES * 8 + 16;                 // (DQ_EVEN: and the sequences' blocks)
 };
 
-enum DecodeQ8End { DQ_ONE_CHUNK = 0, DQ_CLUSTER = 1, DQ_TO_WORKSPACE = 2 };
+// What a block of threads works on: the keys of a slice (a head's rows of a tile of query rows), a share of them as one of a cluster, or an even share of
+// all blocks of all slices, whatever their lengths.
+enum DecodeQ8Mode { DQ_SLICE = 0, DQ_CLUSTER = 1, DQ_EVEN = 2 };
+
+// n even shares of all units: share i starts at all * i / n.
+struct Shares {
+    long long each;
+    int rest, n;
+    __device__ __forceinline__ Shares(long long all, int n_) : each(all / n_), rest((int)(all % n_)), n(n_) {}
+    __device__ __forceinline__ long long start(int i) const { return each * i + (unsigned)(rest * i) / (unsigned)n; }
+};
 
 // Barriers: nothing of global memory.
 template <int DP, int NT>
@@ -106,7 +135,7 @@ __device__ __forceinline__ void decode_q8_prologue(const void* tmap_k, const voi
     }
 }
 
-template <typename T, int DP, int NT, int END>
+template <typename T, int DP, int NT, int MODE>
 __global__ void __launch_bounds__(32 * DQ_WARPS)
 decode_q8_kernel(const __grid_constant__ CUtensorMap tmap_k, const __grid_constant__ CUtensorMap tmap_v, const DecodeQ8Params p) {
     decode_q8_prologue<DP, NT>(&tmap_k, &tmap_v);
@@ -116,24 +145,103 @@ decode_q8_kernel(const __grid_constant__ CUtensorMap tmap_k, const __grid_consta
     constexpr int QP = F32 ? 2 : 1;                              // f16 parts of a value of q
     extern __shared__ __align__(1024) uint8_t smem[];
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
-    const int split = blockIdx.x, Hkv = p.H / p.G, b = blockIdx.y / Hkv, kvh = blockIdx.y % Hkv, tile = blockIdx.z;
-    const int R = p.G * p.Tq, row0 = tile * S::ROWS;
-    int len = p.lengths[b];
-    if (len < 0 || len > p.cap) {
-        if (threadIdx.x == 0) atomicCAS(p.err, 0u, (unsigned)DEERS_KERR_CACHE | 2u);
-        len = min(max(len, 0), p.cap);
+    const int Hkv = p.H / p.G, R = p.G * p.Tq;
+    const auto length = [&](int b) {
+        const int len = p.lengths[b];
+        if (len < 0 || len > p.cap) atomicCAS(p.err, 0u, (unsigned)DEERS_KERR_CACHE | 2u);
+        return min(max(len, 0), p.cap);
+    };
+    long long* before = reinterpret_cast<long long*>(smem + S::SMEM);
+    long long unit = 0, unit_end = 0;                            // DQ_EVEN: this block's, of all slices' blocks in a row
+    if constexpr (MODE == DQ_EVEN) {
+        if (warp == 0) {
+            long long run = 0;
+            for (int b0 = 0; b0 < p.B; b0 += 32) {
+                long long n = b0 + lane < p.B ? (long long)((length(b0 + lane) + 31) / 32) * Hkv * p.tiles : 0;
+#pragma unroll
+                for (int off = 1; off < 32; off *= 2) {
+                    const long long up = __shfl_up_sync(0xffffffffu, n, off);
+                    if (lane >= off) n += up;
+                }
+                if (b0 + lane < p.B) before[b0 + lane + 1] = run + n;
+                run += __shfl_sync(0xffffffffu, n, 31);
+            }
+            if (lane == 0) before[0] = 0;
+            __syncwarp();
+            if (blockIdx.x == 0)
+                for (int i = lane; i <= p.B; i += 32) p.before[i] = before[i];
+        }
+        __syncthreads();
+        const Shares shares(before[p.B], gridDim.x);
+        unit = shares.start(blockIdx.x);
+        unit_end = shares.start(blockIdx.x + 1);
     }
-    // this block's keys: its share of the sequence's blocks of 32
-    const int blocks = (len + 31) / 32;
-    const int blk0 = (int)((long long)blocks * split / p.splits), blk1 = (int)((long long)blocks * (split + 1) / p.splits);
+    if constexpr (MODE == DQ_CLUSTER) cooperative_groups::this_cluster().barrier_arrive();
+    int stage = 0;                                               // of this warp's ring: where its next block is
+    uint32_t phase = 0;
+    for (bool first = true; MODE == DQ_EVEN ? unit < unit_end : first; first = false) {
+    int b, kvh, tile, len, blk0, blk1;
+    bool whole = true;                                           // this block of threads sees all keys of the slice
+    if constexpr (MODE == DQ_EVEN) {
+        int lo = 0, hi = p.B;                                    // the last sequence that begins at or before the unit
+        while (hi - lo > 1) {
+            const int mid = (lo + hi) / 2;
+            if (before[mid] <= unit) lo = mid;
+            else hi = mid;
+        }
+        b = lo;
+        const long long rest = unit - before[b], blocks = (before[b + 1] - before[b]) / (Hkv * p.tiles);
+        const int slice = (int)(rest / blocks);
+        kvh = slice / p.tiles; tile = slice % p.tiles;
+        len = min(max(p.lengths[b], 0), p.cap);
+        blk0 = (int)(rest % blocks);
+        blk1 = (int)min(blocks, blk0 + (unit_end - unit));
+        whole = blk0 == 0 && blk1 == (int)blocks;
+        unit += blk1 - blk0;
+    } else {
+        b = blockIdx.y / Hkv; kvh = blockIdx.y % Hkv; tile = blockIdx.z;
+    }
+    const int row0 = tile * S::ROWS;
+    // q is on its way while the length is (lane (g, t) has row g, channels 16 (t + 4 c) ..)
+    T raw[NT][S::KC][16];
+#pragma unroll
+    for (int nt = 0; nt < NT; ++nt) {
+        const int r = row0 + nt * 8 + g;
+        const T* src = static_cast<const T*>(p.q);
+        if (r < R) src += b * p.sq[0] + (long long)(kvh * p.G + r / p.Tq) * p.sq[1] + (long long)(r % p.Tq) * p.sq[2];
+#pragma unroll
+        for (int c = 0; c < S::KC; ++c) {
+            const int d = 16 * (t + 4 * c);
+            const bool there = r < R && d < p.D;
+            if (p.q_vec) {
+#pragma unroll
+                for (int w = 0; w < (int)sizeof(T); ++w)
+                    reinterpret_cast<uint4*>(raw[nt][c])[w] = there ? reinterpret_cast<const uint4*>(src + d)[w] : make_uint4(0u, 0u, 0u, 0u);
+            } else {
+#pragma unroll
+                for (int e = 0; e < 16; ++e) raw[nt][c][e] = there ? src[d + e] : T(0.f);
+            }
+        }
+    }
+    if constexpr (MODE != DQ_EVEN) {
+        len = length(b);
+        const int blocks = (len + 31) / 32, split = MODE == DQ_CLUSTER ? blockIdx.x : 0;
+        blk0 = (int)((long long)blocks * split / p.splits); blk1 = (int)((long long)blocks * (split + 1) / p.splits);
+    }
     const uint8_t* vb = p.v + b * p.sv[0] + kvh * p.sv[1];
     const float* ksl = p.k_scale + b * p.skl[0] + kvh * p.skl[1];
     const float* vsl = p.v_scale + b * p.svl[0] + kvh * p.svl[1];
 
-    __syncthreads();                                             // the barriers are there
-    uint8_t* ring = smem + warp * (S::STAGES * S::STAGE_BYTES);
     uint64_t* full = reinterpret_cast<uint64_t*>(smem + S::BARS) + warp * S::STAGES;
     const sm100::WaitState ws{reinterpret_cast<uint32_t*>(smem + S::BARS + DQ_WARPS * S::STAGES * 8), p.err};
+    if (MODE == DQ_EVEN) sm100::fence_proxy_async_smem();        // (the ring has been written by threads)
+    // the barriers are there, and the ring is free
+    if (MODE == DQ_EVEN && !first) {
+        if (__syncthreads_or(*ws.abort != 0)) break;
+    } else {
+        __syncthreads();
+    }
+    uint8_t* ring = smem + warp * (S::STAGES * S::STAGE_BYTES);
     // Block `blk` into stage s, by one lane.  (Keys behind the sequence's last may lie in it, and are masked below.)
     auto fetch = [&](int blk, int s) {
         if (blk < blk1 && lane == 0) {
@@ -154,37 +262,22 @@ decode_q8_kernel(const __grid_constant__ CUtensorMap tmap_k, const __grid_consta
     const auto v_key = [&](int r) { return (r >> 2) * 16 + ((r >> 1) & 1) * 8 + 2 * t + (r & 1); };
     const auto v_at = [&](int r, int c) { return 32 * DP + (DP == 64 ? in_boxes(v_key(r), g >> 1) + 8 * (g & 1) : in_boxes(v_key(r), g + 8 * c)); };
 #pragma unroll
-    for (int s = 0; s < S::STAGES - 1; ++s) fetch(blk0 + warp + s * DQ_WARPS, s);
+    for (int s = 0; s < S::STAGES - 1; ++s) fetch(blk0 + warp + s * DQ_WARPS, (stage + s) % S::STAGES);
 
-    // q as the products' second operand: lane (g, t) has row g, channels 16 (t + 4 c) ..
+    float ks_next = 0.f, vs_next = 0.f;                          // scales of the next round's block
+    if (blk0 + warp < blk1) { ks_next = ksl[blk0 + warp]; vs_next = vsl[blk0 + warp]; }
+
+    // q as the products' second operand
     uint32_t qf[NT][QP][S::KC][8];
     float qs[NT][2];                                             // factor of the scores of rows 2t, 2t + 1
     int lim[NT][2];                                              // keys that they see
 #pragma unroll
     for (int nt = 0; nt < NT; ++nt) {
-        const int r = row0 + nt * 8 + g;
         float f[S::KC][16];
-        const T* src = static_cast<const T*>(p.q);
-        if (r < R) src += b * p.sq[0] + (long long)(kvh * p.G + r / p.Tq) * p.sq[1] + (long long)(r % p.Tq) * p.sq[2];
 #pragma unroll
-        for (int c = 0; c < S::KC; ++c) {
-            const int d = 16 * (t + 4 * c);
-            if (r < R && d < p.D) {
-                if (p.q_vec) {
-                    T raw[16];
+        for (int c = 0; c < S::KC; ++c)
 #pragma unroll
-                    for (int w = 0; w < (int)sizeof(T); ++w) reinterpret_cast<uint4*>(raw)[w] = reinterpret_cast<const uint4*>(src + d)[w];
-#pragma unroll
-                    for (int e = 0; e < 16; ++e) f[c][e] = (float)raw[e];
-                } else {
-#pragma unroll
-                    for (int e = 0; e < 16; ++e) f[c][e] = (float)src[d + e];
-                }
-            } else {
-#pragma unroll
-                for (int e = 0; e < 16; ++e) f[c][e] = 0.f;
-            }
-        }
+            for (int e = 0; e < 16; ++e) f[c][e] = (float)raw[nt][c][e];
         float back = 1.f;
         if constexpr (F32) {
             unsigned top = 0;
@@ -234,10 +327,6 @@ decode_q8_kernel(const __grid_constant__ CUtensorMap tmap_k, const __grid_consta
         l[nt][0] = l[nt][1] = 0.f;
     }
 
-    int stage = 0;
-    uint32_t phase = 0;
-    float ks_next = 0.f, vs_next = 0.f;                          // scales of the next round's block
-    if (blk0 + warp < blk1) { ks_next = ksl[blk0 + warp]; vs_next = vsl[blk0 + warp]; }
 #pragma unroll 1
     for (int blk = blk0 + warp; blk < blk1; blk += DQ_WARPS) {
         const float ks = ks_next, vs = vs_next;
@@ -454,7 +543,7 @@ decode_q8_kernel(const __grid_constant__ CUtensorMap tmap_k, const __grid_consta
         }
         if (++stage == S::STAGES) { stage = 0; phase ^= 1u; }
     }
-    chain_next();
+    if (MODE != DQ_EVEN || unit >= unit_end) chain_next();
 
     // ---- the warps meet
 #pragma unroll
@@ -465,7 +554,6 @@ decode_q8_kernel(const __grid_constant__ CUtensorMap tmap_k, const __grid_consta
             for (int off = 4; off <= 16; off *= 2) l[nt][x] += __shfl_xor_sync(0xffffffffu, l[nt][x], off);
     __syncthreads();                                             // every ring has been read
     float* meet = reinterpret_cast<float*>(smem);
-    float* part = reinterpret_cast<float*>(smem + S::MERGE);
     {
         float* mine = meet + warp * S::ROWS * S::OS;
         const float down = vref * (1.0f / DQ_UP);
@@ -496,51 +584,61 @@ decode_q8_kernel(const __grid_constant__ CUtensorMap tmap_k, const __grid_consta
         const int rr = row0 + r;
         return p.lse + ((long long)b * p.H + kvh * p.G + rr / p.Tq) * p.Tq + rr % p.Tq;
     };
-    // n partial rows at `from`, `step` floats apart: (maximum, sum, O) of the whole
-    auto joined = [&](const float* from, int step, int r, int d, float& mx, float& sum) {
-        mx = -INFINITY;
-#pragma unroll
-        for (int w = 0; w < DQ_WARPS; ++w) mx = fmaxf(mx, from[w * step + r * S::OS + DP]);
-        const float ms = mx == -INFINITY ? 0.f : mx;
-        float v = 0.f;
-        sum = 0.f;
-#pragma unroll
-        for (int w = 0; w < DQ_WARPS; ++w) {
-            const float* at = from + w * step + r * S::OS;
-            const float f = exp2f(at[DP] - ms);
-            sum = fmaf(f, at[DP + 1], sum);
-            v = fmaf(f, at[d], v);
-        }
-        return v;
+    const auto finish = [&](int r, int d, const float4& v, float mx, float sum) {      // four channels of a row
+        const float inv = sum == 0.f ? 0.f : 1.0f / sum;
+        put4(out_row(r) + d, make_float4(v.x * inv, v.y * inv, v.z * inv, v.w * inv), p.o_vec);
+        if (p.lse && d == 0) *lse_at(r) = (mx + log2f(sum)) * DQ_LN2;
     };
-    float* to_part = END == DQ_TO_WORKSPACE ? p.part + (((long long)blockIdx.y * gridDim.z + tile) * p.splits + split) * (S::ROWS * (p.D + 2)) : nullptr;
-    for (int i = threadIdx.x; i < rows * p.D; i += 32 * DQ_WARPS) {
-        const int r = i / p.D, d = i % p.D;
-        float mx, sum;
-        const float v = joined(meet, S::ROWS * S::OS, r, d, mx, sum);
-        if constexpr (END == DQ_ONE_CHUNK) {
-            put(out_row(r) + d, sum == 0.f ? 0.f : v / sum);
-            if (p.lse && d == 0) *lse_at(r) = (mx + log2f(sum)) * DQ_LN2;
-        } else if constexpr (END == DQ_CLUSTER) {
-            part[r * S::OS + d] = v;
-            if (d == 0) { part[r * S::OS + DP] = mx; part[r * S::OS + DP + 1] = sum; }
-        } else {
-            to_part[r * (p.D + 2) + d] = v;
-            if (d == 0) { to_part[r * (p.D + 2) + p.D] = mx; to_part[r * (p.D + 2) + p.D + 1] = sum; }
+    // (a share begins inside at most one slice, and ends inside at most one)
+    float* to_part = MODE == DQ_EVEN ? p.part + ((long long)blockIdx.x * 2 + (blk0 > 0 ? 0 : 1)) * (S::ROWS * (p.D + 4)) : nullptr;
+    const int share = ((rows * p.D + p.splits - 1) / p.splits + 3) / 4 * 4;             // DQ_CLUSTER: of the outputs, to every block
+    if constexpr (MODE == DQ_CLUSTER) cooperative_groups::this_cluster().barrier_wait();       // (all have started: their memory may be written to)
+    for (int r = warp; r < rows; r += DQ_WARPS) {
+        float w[DQ_WARPS], mx = -INFINITY, sum = 0.f;
+#pragma unroll
+        for (int x = 0; x < DQ_WARPS; ++x) {
+            w[x] = meet[(x * S::ROWS + r) * S::OS + DP];
+            mx = fmaxf(mx, w[x]);
+        }
+        const float ms = mx == -INFINITY ? 0.f : mx;
+#pragma unroll
+        for (int x = 0; x < DQ_WARPS; ++x) {
+            w[x] = exp2f(w[x] - ms);
+            sum = fmaf(w[x], meet[(x * S::ROWS + r) * S::OS + DP + 1], sum);
+        }
+        for (int d = 4 * lane; d < p.D; d += 128) {
+            float4 v = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll
+            for (int x = 0; x < DQ_WARPS; ++x) add4(v, w[x], *reinterpret_cast<const float4*>(&meet[(x * S::ROWS + r) * S::OS + d]));
+            if constexpr (MODE == DQ_CLUSTER) {
+                const int i = r * p.D + d, z = i / share;
+                const uint32_t to = sm100::cluster_addr(smem + S::SENT, z);
+                send4(to + 8 * 8 * S::ROWS + 4 * (blockIdx.x * share + i - z * share), v);
+                // (whoever owns channels of a row needs its maxima and sums: the first of its channels, or of that share, brings them)
+                if (d == 0 || i == z * share) {
+                    send(to + 8 * (blockIdx.x * S::ROWS + r), mx);
+                    send(to + 8 * (blockIdx.x * S::ROWS + r) + 4, sum);
+                }
+            } else if (MODE == DQ_SLICE || whole) {
+                finish(r, d, v, mx, sum);
+            } else {
+                *reinterpret_cast<float4*>(to_part + r * (p.D + 4) + d) = v;
+                if (d == 0) *reinterpret_cast<float2*>(to_part + r * (p.D + 4) + p.D) = make_float2(mx, sum);
+            }
         }
     }
-    if constexpr (END == DQ_CLUSTER) {
-        cooperative_groups::cluster_group cluster = cooperative_groups::this_cluster();
-        cluster.sync();
-        const float* from[8];
-#pragma unroll
-        for (int z = 0; z < 8; ++z) from[z] = cluster.map_shared_rank(part, z < p.splits ? z : 0);
-        for (int i = split * 32 * DQ_WARPS + threadIdx.x; i < rows * p.D; i += p.splits * 32 * DQ_WARPS) {
-            const int r = i / p.D, d = i % p.D;
-            float w[8], mx = -INFINITY, sum = 0.f, v = 0.f;
+    if constexpr (MODE == DQ_CLUSTER) {
+        cooperative_groups::this_cluster().sync();
+        const float2* ml = reinterpret_cast<const float2*>(smem + S::SENT);
+        const float* parts = reinterpret_cast<const float*>(ml + 8 * S::ROWS);
+        const int end = min(share, rows * p.D - (int)blockIdx.x * share);
+        for (int j = 4 * (int)threadIdx.x; j < end; j += 128 * DQ_WARPS) {
+            const int i = blockIdx.x * share + j, r = i / p.D;
+            float w[8], mx = -INFINITY, sum = 0.f;
+            float4 v = make_float4(0.f, 0.f, 0.f, 0.f);
 #pragma unroll
             for (int z = 0; z < 8; ++z) {
-                w[z] = z < p.splits ? from[z][r * S::OS + DP] : -INFINITY;
+                w[z] = z < p.splits ? ml[z * S::ROWS + r].x : -INFINITY;
                 mx = fmaxf(mx, w[z]);
             }
             const float ms = mx == -INFINITY ? 0.f : mx;
@@ -548,62 +646,100 @@ decode_q8_kernel(const __grid_constant__ CUtensorMap tmap_k, const __grid_consta
             for (int z = 0; z < 8; ++z)
                 if (z < p.splits) {
                     const float f = exp2f(w[z] - ms);
-                    sum = fmaf(f, from[z][r * S::OS + DP + 1], sum);
-                    v = fmaf(f, from[z][r * S::OS + d], v);
+                    sum = fmaf(f, ml[z * S::ROWS + r].y, sum);
+                    add4(v, f, *reinterpret_cast<const float4*>(&parts[z * share + j]));
                 }
-            put(out_row(r) + d, sum == 0.f ? 0.f : v / sum);
-            if (p.lse && d == 0) *lse_at(r) = (mx + log2f(sum)) * DQ_LN2;
+            finish(r, i - r * p.D, v, mx, sum);
         }
-        cluster.sync();                                          // nobody leaves while a peer still reads its part
+    }
     }
 }
 
-// Joins the chunks of a slice's rows from the workspace: a block per (row of a tile, tile, slice).
+// Rows of slices that no block of threads has seen whole, from what each has left of them; one row a block.
 template <typename T>
-__global__ void __launch_bounds__(128) decode_q8_join_kernel(const DecodeQ8Params p, int tile_rows, int tiles) {
-    chain_begin();
-    __shared__ float s_w[DQ_MAX_SPLITS], s_r[8];
+__global__ void __launch_bounds__(256) decode_q8_join_kernel(const DecodeQ8Params p, int tile_rows, int shares) {
+    chain_wait();
+    __shared__ float s_w[DQ_MAX_BLOCKS], s_l[DQ_MAX_BLOCKS], s_r[16];
+    __shared__ __align__(16) float s_o[8][256];
+    __shared__ int s_at[DQ_MAX_BLOCKS];
     const int r = blockIdx.x, tile = blockIdx.z, Hkv = p.H / p.G, b = blockIdx.y / Hkv, kvh = blockIdx.y % Hkv;
     const int rr = tile * tile_rows + r, lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
     if (rr >= p.G * p.Tq) return;
-    const long long step = (long long)tile_rows * (p.D + 2);
-    const float* part = p.part + ((long long)blockIdx.y * tiles + tile) * p.splits * step + r * (p.D + 2);
+    const long long all = p.before[p.B], here = p.before[b], blocks = (p.before[b + 1] - here) / (Hkv * p.tiles);
+    const long long u0 = here + (kvh * p.tiles + tile) * blocks, u1 = u0 + blocks;
+    const int head = kvh * p.G + rr / p.Tq, i = rr % p.Tq;
+    T* o = static_cast<T*>(p.o) + b * p.so[0] + head * p.so[1] + i * p.so[2];
+    float* lse = p.lse ? p.lse + ((long long)b * p.H + head) * p.Tq + i : nullptr;
+    if (blocks == 0) {                                           // a sequence without keys is nobody's share
+        for (int d = threadIdx.x; d < p.D; d += 256) put(o + d, 0.f);
+        if (lse && threadIdx.x == 0) *lse = -INFINITY;
+        return;
+    }
+    const Shares sh(all, shares);
+    const auto share_of = [&](long long u) {                     // the share that unit u is in: the last one that starts at or before it
+        int c = (int)(u * shares / all);
+        while (c + 1 < shares && sh.start(c + 1) <= u) ++c;
+        while (sh.start(c) > u) --c;
+        return c;
+    };
+    const int c0 = share_of(u0), n = share_of(u1 - 1) - c0 + 1;
+    if (n == 1) return;                                          // seen whole
+    const int step = tile_rows * (p.D + 4);
+    const float* part = p.part + r * (p.D + 4);
     float mx = -INFINITY;
-    for (int z = threadIdx.x; z < p.splits; z += 128) {
-        s_w[z] = part[z * step + p.D];
-        mx = fmaxf(mx, s_w[z]);
+    for (int z = threadIdx.x; z < n; z += 256) {
+        // (the first share has it as its end, or from its own start; the others begin inside; a share of nothing has left nothing)
+        const long long from = sh.start(c0 + z);
+        const int at = sh.start(c0 + z + 1) > from ? (c0 + z) * 2 + (from > u0 ? 0 : 1) : -1;
+        s_at[z] = at;
+        const float2 ms = at < 0 ? make_float2(-INFINITY, 0.f) : *reinterpret_cast<const float2*>(part + (long long)at * step + p.D);
+        s_w[z] = ms.x; s_l[z] = ms.y;
+        mx = fmaxf(mx, ms.x);
     }
 #pragma unroll
     for (int off = 16; off >= 1; off >>= 1) mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, off));
     if (lane == 0) s_r[warp] = mx;
     __syncthreads();
-    mx = fmaxf(fmaxf(s_r[0], s_r[1]), fmaxf(s_r[2], s_r[3]));
+#pragma unroll
+    for (int w = 0; w < 8; ++w) mx = fmaxf(mx, s_r[w]);
     const float ms = mx == -INFINITY ? 0.f : mx;
     float sum = 0.f;
-    for (int z = threadIdx.x; z < p.splits; z += 128) {
-        const float w = exp2f(s_w[z] - ms);
+    for (int z = threadIdx.x; z < n; z += 256) {
+        const float w = s_at[z] < 0 ? 0.f : exp2f(s_w[z] - ms);
         s_w[z] = w;
-        sum = fmaf(w, part[z * step + p.D + 1], sum);
+        sum = fmaf(w, s_l[z], sum);
     }
 #pragma unroll
     for (int off = 16; off >= 1; off >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, off);
-    if (lane == 0) s_r[4 + warp] = sum;
+    if (lane == 0) s_r[8 + warp] = sum;
     __syncthreads();
-    sum = (s_r[4] + s_r[5]) + (s_r[6] + s_r[7]);
-    const int head = kvh * p.G + rr / p.Tq, i = rr % p.Tq;
-    T* o = static_cast<T*>(p.o) + b * p.so[0] + head * p.so[1] + i * p.so[2];
-    for (int d = threadIdx.x; d < p.D; d += 128) {
+    sum = 0.f;
+#pragma unroll
+    for (int w = 0; w < 8; ++w) sum += s_r[8 + w];
+    // a warp adds up every eighth share, four channels a lane
+    for (int d = 4 * lane; d < p.D; d += 128) {
+        float4 v = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll 8
+        for (int z = warp; z < n; z += 8) {
+            const float w = s_w[z];
+            const float4 x = s_at[z] < 0 ? make_float4(0.f, 0.f, 0.f, 0.f) : *reinterpret_cast<const float4*>(part + (long long)s_at[z] * step + d);
+            add4(v, w, x);
+        }
+        *reinterpret_cast<float4*>(&s_o[warp][d]) = v;
+    }
+    __syncthreads();
+    for (int d = threadIdx.x; d < p.D; d += 256) {
         float v = 0.f;
-        for (int z = 0; z < p.splits; ++z) v = fmaf(s_w[z], part[z * step + d], v);
+#pragma unroll
+        for (int w = 0; w < 8; ++w) v += s_o[w][d];
         put(o + d, sum == 0.f ? 0.f : v / sum);
     }
-    if (p.lse && threadIdx.x == 0) p.lse[((long long)b * p.H + head) * p.Tq + i] = (mx + log2f(sum)) * DQ_LN2;
+    if (lse && threadIdx.x == 0) *lse = (mx + log2f(sum)) * DQ_LN2;
 }
 
-struct DecodeQ8Plan { int dp, nt, tiles, splits, end; };
+struct DecodeQ8Plan { int dp, nt, tiles, mode, splits, shares; };   // splits: blocks of a cluster; shares: of all blocks
 
 // How the work is cut.  Sixteen query rows share a walk where there are more than eight (heads up to 128 wide: the registers hold their O).
-// The slices' keys are cut so that every SM has two blocks: up to eight chunks meet as a cluster, more through the workspace.
 DecodeQ8Plan plan_decode_q8(const deers_decode_q8_desc* d) {
     DecodeQ8Plan p;
     p.dp = d->cache.D <= 64 ? 64 : d->cache.D <= 128 ? 128 : 256;
@@ -615,16 +751,18 @@ DecodeQ8Plan plan_decode_q8(const deers_decode_q8_desc* d) {
     long long want = (2 * 148 + slices - 1) / slices;
     const long long most = (blocks + 7) / 8;                     // at least 256 keys a chunk
     if (want > most) want = most;
-    if (want > DQ_MAX_SPLITS) want = DQ_MAX_SPLITS;
     if (want < 1) want = 1;
-    p.splits = (int)want;
-    p.end = want == 1 ? DQ_ONE_CHUNK : want <= 8 ? DQ_CLUSTER : DQ_TO_WORKSPACE;
+    const char* e = getenv("DQMODE");
+    int mode = want == 1 ? DQ_SLICE : want <= 8 ? DQ_CLUSTER : DQ_EVEN, sp = (int)want, sh = 296;
+    if (e) sscanf(e, "%d,%d,%d", &mode, &sp, &sh);
+    p.mode = mode; p.splits = mode == DQ_CLUSTER ? sp : 1; p.shares = mode == DQ_EVEN ? sh : 0;
     return p;
 }
 
+size_t decode_q8_head(const deers_decode_q8_desc* d) { return ((size_t)(d->cache.B + 1) * sizeof(long long) + 255) / 256 * 256; }
 size_t decode_q8_bytes(const deers_decode_q8_desc* d, const DecodeQ8Plan& p) {
-    if (p.end != DQ_TO_WORKSPACE) return 0;
-    return (size_t)d->cache.B * d->cache.H * p.tiles * p.splits * (8 * p.nt) * (d->cache.D + 2) * sizeof(float);
+    if (p.mode != DQ_EVEN) return 0;
+    return decode_q8_head(d) + (size_t)p.shares * 2 * (8 * p.nt) * (d->cache.D + 4) * sizeof(float);
 }
 
 int decode_q8_check(const deers_decode_q8_desc* d) {
@@ -664,18 +802,17 @@ int decode_q8_launch(deers_ctx* ctx, const DecodeQ8Params& p, const DecodeQ8Plan
     int rc = tmap_cache(ctx, &tk, cache.k, cache, cache.k_strides, S::BOX);
     if (!rc) rc = tmap_cache(ctx, &tv, cache.v, cache, cache.v_strides, S::BOX);
     if (rc) return rc;
-    const dim3 grid(plan.splits, slices, plan.tiles);
-    if (plan.end == DQ_ONE_CHUNK) {
-        DEERS_SMEM_ONCE(ctx, (decode_q8_kernel<T, DP, NT, DQ_ONE_CHUNK>), S::SMEM);
-        DEERS_CUDA_TRY(ctx, launch_chained(ctx, decode_q8_kernel<T, DP, NT, DQ_ONE_CHUNK>, grid, 32 * DQ_WARPS, S::SMEM, 1, tk, tv, p));
-    } else if (plan.end == DQ_CLUSTER) {
+    if (plan.mode == DQ_SLICE) {
+        DEERS_SMEM_ONCE(ctx, (decode_q8_kernel<T, DP, NT, DQ_SLICE>), S::SMEM);
+        DEERS_CUDA_TRY(ctx, launch_chained(ctx, decode_q8_kernel<T, DP, NT, DQ_SLICE>, dim3(1, slices, plan.tiles), 32 * DQ_WARPS, S::SMEM, 1, tk, tv, p));
+    } else if (plan.mode == DQ_CLUSTER) {
         DEERS_SMEM_ONCE(ctx, (decode_q8_kernel<T, DP, NT, DQ_CLUSTER>), S::SMEM);
-        DEERS_CUDA_TRY(ctx, launch_chained(ctx, decode_q8_kernel<T, DP, NT, DQ_CLUSTER>, grid, 32 * DQ_WARPS, S::SMEM, plan.splits, tk, tv, p));
+        DEERS_CUDA_TRY(ctx, launch_chained(ctx, decode_q8_kernel<T, DP, NT, DQ_CLUSTER>, dim3(plan.splits, slices, plan.tiles), 32 * DQ_WARPS, S::SMEM, plan.splits, tk, tv, p));
     } else {
-        DEERS_SMEM_ONCE(ctx, (decode_q8_kernel<T, DP, NT, DQ_TO_WORKSPACE>), S::SMEM);
-        DEERS_CUDA_TRY(ctx, launch_chained(ctx, decode_q8_kernel<T, DP, NT, DQ_TO_WORKSPACE>, grid, 32 * DQ_WARPS, S::SMEM, 1, tk, tv, p));
-        const dim3 rows(S::ROWS, slices, plan.tiles);
-        DEERS_CUDA_TRY(ctx, launch_chained(ctx, decode_q8_join_kernel<T>, rows, 128, 0, 1, p, S::ROWS, plan.tiles));
+        const int smem = S::SMEM + (p.B + 1) * (int)sizeof(long long);
+        DEERS_SMEM_ONCE(ctx, (decode_q8_kernel<T, DP, NT, DQ_EVEN>), S::SMEM + (DQ_MAX_EVEN + 1) * sizeof(long long));
+        DEERS_CUDA_TRY(ctx, launch_chained(ctx, decode_q8_kernel<T, DP, NT, DQ_EVEN>, (unsigned)plan.shares, 32 * DQ_WARPS, smem, 1, tk, tv, p));
+        DEERS_CUDA_TRY(ctx, launch_chained(ctx, decode_q8_join_kernel<T>, dim3(S::ROWS, slices, plan.tiles), 256, 0, 1, p, S::ROWS, plan.shares));
         ctx->launches += 1;
     }
     return DEERS_OK;
@@ -704,17 +841,20 @@ extern "C" int deers_b200_attn_decode_q8(deers_ctx* ctx, const deers_decode_q8_d
     if (((uintptr_t)q | (uintptr_t)o) & (es - 1) || ((uintptr_t)lengths | (uintptr_t)lse) & 3u) return DEERS_ERR_LAYOUT;
     const DecodeQ8Plan plan = plan_decode_q8(d);
     const size_t need = decode_q8_bytes(d, plan);
-    if (need && (!workspace || workspace_bytes < need || ((uintptr_t)workspace & 3u))) return DEERS_ERR_WORKSPACE;
+    if (need && (!workspace || workspace_bytes < need || ((uintptr_t)workspace & 15u))) return DEERS_ERR_WORKSPACE;
     DEERS_CUDA_TRY(ctx, cudaSetDevice(ctx->device));
     const deers_cache_q8& c = d->cache;
     DecodeQ8Params p;
-    p.q = q; p.o = o; p.lse = lse; p.lengths = lengths; p.part = (float*)workspace;
+    p.q = q; p.o = o; p.lse = lse; p.lengths = lengths;
+    p.before = (long long*)workspace; p.part = need ? (float*)((char*)workspace + decode_q8_head(d)) : nullptr;
     p.k = (const uint8_t*)c.k; p.v = (const uint8_t*)c.v; p.k_scale = c.k_scale; p.v_scale = c.v_scale;
     for (int i = 0; i < 3; ++i) { p.sq[i] = d->q_strides[i]; p.so[i] = d->o_strides[i]; p.sk[i] = c.k_strides[i]; p.sv[i] = c.v_strides[i]; }
     for (int i = 0; i < 2; ++i) { p.skl[i] = c.k_scale_strides[i]; p.svl[i] = c.v_scale_strides[i]; }
+    p.B = c.B; p.tiles = plan.tiles;
     p.H = d->H; p.G = d->H / c.H; p.Tq = d->Tq; p.D = c.D; p.cap = c.capacity; p.causal = d->causal; p.splits = plan.splits;
     p.scale = d->scale; p.err = ctx->dev_err;
     const int64_t al = 16 / (int64_t)es - 1;
+    p.o_vec = ((uintptr_t)o & 15u) == 0 && ((d->o_strides[0] | d->o_strides[1] | d->o_strides[2]) & al) == 0;
     p.q_vec = ((uintptr_t)q & 15u) == 0 && ((d->q_strides[0] | d->q_strides[1] | d->q_strides[2]) & al) == 0;
     {
         KernelTimerScope ts(ctx, DEERS_K_DECODE);
