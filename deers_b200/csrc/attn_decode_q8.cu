@@ -25,14 +25,14 @@
 #include "tma_host.cuh"
 
 #include <cooperative_groups.h>
-#include <stdlib.h>
 
 int deers_check_cache(const deers_cache_q8* c);
 
 namespace {
 
 constexpr int DQ_WARPS = 4;
-constexpr int DQ_MAX_BLOCKS = 3 * 148, DQ_MAX_EVEN = 256;        // blocks of threads and sequences of an even share
+constexpr int DQ_MAX_SHARES = 2 * 148, DQ_MAX_EVEN = 256;        // even shares: blocks of threads and sequences at most
+constexpr int DQ_LONG = 16384;                                   // keys a slice can hold from which on shares are even
 constexpr float DQ_LOG2E = 1.4426950408889634f, DQ_LN2 = 0.6931471805599453f;
 constexpr float DQ_UP = 32768.0f;                                // weights are at most 2^15 of f16's 65504
 
@@ -89,15 +89,17 @@ __device__ __forceinline__ void put4(__half* p, const float4& v, int vec) {
     else { put(p, v.x); put(p + 1, v.y); put(p + 2, v.z); put(p + 3, v.w); }
 }
 
-// Shapes of a kernel for heads of up to DP channels and 8 * NT query rows.
+// Shapes of a kernel for heads of up to DP channels (32, 64, 96, 128 or 256) and 8 * NT query rows.
+//   K: a lane (g, t) has the channels 16 (t + 4 c) .. + 15 of a key, c < KC, and of DP = 32 or 96 the last 32's 8 t .. + 7: four to a product step
+//   V: the channels VB (g + 8 c) .. + VB - 1, c < VC, and the last 32's 4 g .. + 3: two to a product tile
 template <int DP, int NT>
 struct Shape {
-    static constexpr int KC = DP / 64;                           // 16-byte pieces of a key that a lane owns: at 16 * (lane % 4 + 4 c)
-    static constexpr int VB = DP >= 128 ? 16 : 8;                // bytes of a piece of V: at VB * (lane / 4 + 8 c)
-    static constexpr int VC = DP / 8 / VB;
-    static constexpr int STAGES = DP == 64 ? 4 : 2;
-    static constexpr int STAGE_BYTES = 32 * 2 * DP;              // 32 keys, K and V
-    static constexpr int BOX = DP == 64 ? 64 : 128, BOXES = DP / BOX;     // bytes of a key in a box of 32 keys, boxes of K or of V
+    static constexpr bool TAIL = DP % 64 != 0;
+    static constexpr int KC = DP / 64, KS = DP / 16;             // 16-byte pieces; steps
+    static constexpr int VB = DP % 128 == 0 ? 16 : 8, VC = (DP - 32 * TAIL) / 8 / VB, VT = DP / 16;      // bytes of a piece, pieces; tiles
+    static constexpr int BOX = DP <= 64 ? 64 : 128, BOXES = DP == 256 ? 2 : 1;       // bytes of a key in a box of 32 keys (zeros behind D), boxes of K or of V
+    static constexpr int HALF_STAGE = 32 * BOX * BOXES, STAGE_BYTES = 2 * HALF_STAGE;         // K, V
+    static constexpr int STAGES = DP <= 64 ? 4 : 2;
     static constexpr int RING = DQ_WARPS * STAGES * STAGE_BYTES;
     static constexpr int ROWS = 8 * NT;
     static constexpr int OS = DP + 4;                            // row of partial results: O, then maximum and sum
@@ -106,6 +108,11 @@ struct Shape {
     // (the ring has been read when the warps meet; what other blocks of a cluster send has a place of its own)
     static constexpr int SENT = RING > MERGE ? RING : MERGE, BARS = SENT + 8 * ROWS * 8 + PART + 8 * 32;
     static constexpr int SMEM = BARS + DQ_WARPS * STAGES * 8 + 16;                 // (DQ_EVEN: and the sequences' blocks)
+    // first of the four channels of product step i, of the two channels of tile j (a tile's rows 8 to 15 are the next ones)
+    static __device__ __forceinline__ int k_channel(int i, int t) { return i < 4 * KC ? 16 * (t + 4 * (i / 4)) + 4 * (i % 4) : DP - 32 + 8 * t + 4 * (i - 4 * KC); }
+    static __device__ __forceinline__ int v_channel(int j, int g) {
+        return j < VC * (VB / 2) ? VB * (g + 8 * (j / (VB / 2))) + 2 * (j % (VB / 2)) : DP - 32 + 4 * g + 2 * (j - VC * (VB / 2));
+    }
 };
 
 // What a block of threads works on: the keys of a slice (a head's rows of a tile of query rows), a share of them as one of a cluster, or an even share of
@@ -203,23 +210,23 @@ decode_q8_kernel(const __grid_constant__ CUtensorMap tmap_k, const __grid_consta
     }
     const int row0 = tile * S::ROWS;
     // q is on its way while the length is (lane (g, t) has row g, channels 16 (t + 4 c) ..)
-    T raw[NT][S::KC][16];
+    alignas(16) T raw[NT][S::KS][4];
 #pragma unroll
     for (int nt = 0; nt < NT; ++nt) {
         const int r = row0 + nt * 8 + g;
         const T* src = static_cast<const T*>(p.q);
         if (r < R) src += b * p.sq[0] + (long long)(kvh * p.G + r / p.Tq) * p.sq[1] + (long long)(r % p.Tq) * p.sq[2];
 #pragma unroll
-        for (int c = 0; c < S::KC; ++c) {
-            const int d = 16 * (t + 4 * c);
+        for (int i = 0; i < S::KS; i += 2) {                     // eight channels
+            const int d = S::k_channel(i, t);
             const bool there = r < R && d < p.D;
             if (p.q_vec) {
 #pragma unroll
-                for (int w = 0; w < (int)sizeof(T); ++w)
-                    reinterpret_cast<uint4*>(raw[nt][c])[w] = there ? reinterpret_cast<const uint4*>(src + d)[w] : make_uint4(0u, 0u, 0u, 0u);
+                for (int w = 0; w < (int)sizeof(T) / 2; ++w)
+                    reinterpret_cast<uint4*>(raw[nt][i])[w] = there ? reinterpret_cast<const uint4*>(src + d)[w] : make_uint4(0u, 0u, 0u, 0u);
             } else {
 #pragma unroll
-                for (int e = 0; e < 16; ++e) raw[nt][c][e] = there ? src[d + e] : T(0.f);
+                for (int e = 0; e < 8; ++e) raw[nt][i + e / 4][e % 4] = there ? src[d + e] : T(0.f);
             }
         }
     }
@@ -249,18 +256,28 @@ decode_q8_kernel(const __grid_constant__ CUtensorMap tmap_k, const __grid_consta
 #pragma unroll
             for (int i = 0; i < S::BOXES; ++i) {
                 sm100::tma_load_4d(ring + s * S::STAGE_BYTES + i * 32 * S::BOX, &tmap_k, &full[s], i * S::BOX, blk * 32, kvh, b);
-                sm100::tma_load_4d(ring + s * S::STAGE_BYTES + 32 * DP + i * 32 * S::BOX, &tmap_v, &full[s], i * S::BOX, blk * 32, kvh, b);
+                sm100::tma_load_4d(ring + s * S::STAGE_BYTES + S::HALF_STAGE + i * 32 * S::BOX, &tmap_v, &full[s], i * S::BOX, blk * 32, kvh, b);
             }
         }
     };
-    // 16 bytes of key j at 16 * piece (bytes 8 * half of them) inside the boxes of K or of V
-    auto in_boxes = [&](int j, int piece) {
-        if constexpr (DP == 64) return j * 64 + ((piece ^ (j >> 1 & 3)) << 4);
-        else return (piece >> 3) * (32 * 128) + j * 128 + (((piece & 7) ^ (j & 7)) << 4);
+    // Place of channel d of key j inside the boxes of K or of V (16-byte pieces lie swizzled)
+    auto in_boxes = [&](int j, int d) {
+        if constexpr (S::BOX == 64) return j * 64 + (((d >> 4) ^ (j >> 1 & 3)) << 4) + (d & 15);
+        else return (d >> 7) * (32 * 128) + j * 128 + ((((d >> 4) & 7) ^ (j & 7)) << 4) + (d & 15);
     };
     // This lane's keys of a block: 8 r + g of K; 2t, 2t + 1, 2t + 8, 2t + 9 of either half of V.
     const auto v_key = [&](int r) { return (r >> 2) * 16 + ((r >> 1) & 1) * 8 + 2 * t + (r & 1); };
-    const auto v_at = [&](int r, int c) { return 32 * DP + (DP == 64 ? in_boxes(v_key(r), g >> 1) + 8 * (g & 1) : in_boxes(v_key(r), g + 8 * c)); };
+    const auto v_piece = [&](const uint8_t* st, int r, int d, auto& w) {
+        const uint8_t* at = st + S::HALF_STAGE + in_boxes(v_key(r), d);
+        if constexpr (sizeof(w) == 16) *reinterpret_cast<uint4*>(w) = *reinterpret_cast<const uint4*>(at);
+        else if constexpr (sizeof(w) == 8) *reinterpret_cast<uint2*>(w) = *reinterpret_cast<const uint2*>(at);
+        else w[0] = *reinterpret_cast<const uint32_t*>(at);
+    };
+    const auto k_words = [&](const uint8_t* st, int j, uint32_t (&w)[S::KS]) {
+#pragma unroll
+        for (int c = 0; c < S::KC; ++c) *reinterpret_cast<uint4*>(w + 4 * c) = *reinterpret_cast<const uint4*>(st + in_boxes(j, 16 * (t + 4 * c)));
+        if constexpr (S::TAIL) *reinterpret_cast<uint2*>(w + 4 * S::KC) = *reinterpret_cast<const uint2*>(st + in_boxes(j, DP - 32 + 8 * t));
+    };
 #pragma unroll
     for (int s = 0; s < S::STAGES - 1; ++s) fetch(blk0 + warp + s * DQ_WARPS, (stage + s) % S::STAGES);
 
@@ -268,43 +285,35 @@ decode_q8_kernel(const __grid_constant__ CUtensorMap tmap_k, const __grid_consta
     if (blk0 + warp < blk1) { ks_next = ksl[blk0 + warp]; vs_next = vsl[blk0 + warp]; }
 
     // q as the products' second operand
-    uint32_t qf[NT][QP][S::KC][8];
+    uint32_t qf[NT][QP][S::KS][2];
     float qs[NT][2];                                             // factor of the scores of rows 2t, 2t + 1
     int lim[NT][2];                                              // keys that they see
 #pragma unroll
     for (int nt = 0; nt < NT; ++nt) {
-        float f[S::KC][16];
-#pragma unroll
-        for (int c = 0; c < S::KC; ++c)
-#pragma unroll
-            for (int e = 0; e < 16; ++e) f[c][e] = (float)raw[nt][c][e];
-        float back = 1.f;
+        float back = 1.f, up = 1.f;
         if constexpr (F32) {
             unsigned top = 0;
 #pragma unroll
-            for (int c = 0; c < S::KC; ++c)
+            for (int i = 0; i < S::KS; ++i)
 #pragma unroll
-                for (int e = 0; e < 16; ++e) top = max(top, __float_as_uint(f[c][e]) & 0x7fffffffu);
+                for (int e = 0; e < 4; ++e) top = max(top, __float_as_uint((float)raw[nt][i][e]) & 0x7fffffffu);
             top = max(top, __shfl_xor_sync(0xffffffffu, top, 1));
             top = max(top, __shfl_xor_sync(0xffffffffu, top, 2));
             // a power of two that brings the largest value to 2^14 .. 2^15 (exponents of factor and inverse both in range)
             int e = 141 - (int)(top >> 23);
             e = top == 0 || top >= 0x7f800000u ? 0 : max(-100, min(100, e));
-            const float up = __uint_as_float((unsigned)(127 + e) << 23);
+            up = __uint_as_float((unsigned)(127 + e) << 23);
             back = __uint_as_float((unsigned)(127 - e) << 23);
-#pragma unroll
-            for (int c = 0; c < S::KC; ++c)
-#pragma unroll
-                for (int k = 0; k < 16; ++k) f[c][k] *= up;
         }
 #pragma unroll
-        for (int c = 0; c < S::KC; ++c)
+        for (int i = 0; i < S::KS; ++i)
 #pragma unroll
-            for (int w = 0; w < 8; ++w) {
-                qf[nt][0][c][w] = pack2(f[c][2 * w], f[c][2 * w + 1]);
+            for (int w = 0; w < 2; ++w) {
+                const float x = (float)raw[nt][i][2 * w] * up, y = (float)raw[nt][i][2 * w + 1] * up;
+                qf[nt][0][i][w] = pack2(x, y);
                 if constexpr (F32) {
-                    const float2 hi = unpack2(qf[nt][0][c][w]);
-                    qf[nt][1][c][w] = pack2(f[c][2 * w] - hi.x, f[c][2 * w + 1] - hi.y);
+                    const float2 hi = unpack2(qf[nt][0][i][w]);
+                    qf[nt][1][i][w] = pack2(x - hi.x, y - hi.y);
                 }
             }
 #pragma unroll
@@ -316,11 +325,11 @@ decode_q8_kernel(const __grid_constant__ CUtensorMap tmap_k, const __grid_consta
     }
     const int lim_min = p.causal ? len - (p.Tq - 1) : len;       // keys that every row sees
 
-    float o[NT][DP / 16][4], m[NT][2], l[NT][2], vref = 0.f;
+    float o[NT][S::VT][4], m[NT][2], l[NT][2], vref = 0.f;
 #pragma unroll
     for (int nt = 0; nt < NT; ++nt) {
 #pragma unroll
-        for (int j = 0; j < DP / 16; ++j)
+        for (int j = 0; j < S::VT; ++j)
 #pragma unroll
             for (int e = 0; e < 4; ++e) o[nt][j][e] = 0.f;
         m[nt][0] = m[nt][1] = -INFINITY;
@@ -340,7 +349,7 @@ decode_q8_kernel(const __grid_constant__ CUtensorMap tmap_k, const __grid_consta
         float s[NT][2][4];
 #pragma unroll
         for (int mt = 0; mt < 2; ++mt) {
-            constexpr int CHAINS = F32 ? S::KC + 1 : 1;
+            constexpr int CHAINS = F32 ? (S::KS + 3) / 4 + 1 : 1;
             float sum[NT][CHAINS][4];
 #pragma unroll
             for (int nt = 0; nt < NT; ++nt)
@@ -348,19 +357,16 @@ decode_q8_kernel(const __grid_constant__ CUtensorMap tmap_k, const __grid_consta
                 for (int i = 0; i < CHAINS; ++i)
 #pragma unroll
                     for (int e = 0; e < 4; ++e) sum[nt][i][e] = 0.f;
+            uint32_t xw[S::KS], yw[S::KS];
+            k_words(st, 16 * mt + g, xw);
+            k_words(st, 16 * mt + 8 + g, yw);
 #pragma unroll
-            for (int c = 0; c < S::KC; ++c) {
-                const uint4 x = *reinterpret_cast<const uint4*>(st + in_boxes(16 * mt + g, t + 4 * c));
-                const uint4 y = *reinterpret_cast<const uint4*>(st + in_boxes(16 * mt + 8 + g, t + 4 * c));
-                const uint32_t xw[4] = {x.x, x.y, x.z, x.w}, yw[4] = {y.x, y.y, y.z, y.w};
+            for (int i = 0; i < S::KS; ++i) {
+                const uint32_t a0 = q8::e4m3_lo(xw[i]), a2 = q8::e4m3_hi(xw[i]), a1 = q8::e4m3_lo(yw[i]), a3 = q8::e4m3_hi(yw[i]);
 #pragma unroll
-                for (int w = 0; w < 4; ++w) {
-                    const uint32_t a0 = q8::e4m3_lo(xw[w]), a2 = q8::e4m3_hi(xw[w]), a1 = q8::e4m3_lo(yw[w]), a3 = q8::e4m3_hi(yw[w]);
-#pragma unroll
-                    for (int nt = 0; nt < NT; ++nt) {
-                        mma16816(sum[nt][F32 ? c : 0], a0, a1, a2, a3, qf[nt][0][c][2 * w], qf[nt][0][c][2 * w + 1]);
-                        if constexpr (F32) mma16816(sum[nt][S::KC], a0, a1, a2, a3, qf[nt][1][c][2 * w], qf[nt][1][c][2 * w + 1]);
-                    }
+                for (int nt = 0; nt < NT; ++nt) {
+                    mma16816(sum[nt][F32 ? i / 4 : 0], a0, a1, a2, a3, qf[nt][0][i][0], qf[nt][0][i][1]);
+                    if constexpr (F32) mma16816(sum[nt][CHAINS - 1], a0, a1, a2, a3, qf[nt][1][i][0], qf[nt][1][i][1]);
                 }
             }
 #pragma unroll
@@ -421,7 +427,7 @@ decode_q8_kernel(const __grid_constant__ CUtensorMap tmap_k, const __grid_consta
 #pragma unroll
             for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
-                for (int j = 0; j < DP / 16; ++j)
+                for (int j = 0; j < S::VT; ++j)
 #pragma unroll
                     for (int e = 0; e < 4; ++e) o[nt][j][e] *= fac[nt][e & 1] * vfac;
         }
@@ -443,20 +449,24 @@ decode_q8_kernel(const __grid_constant__ CUtensorMap tmap_k, const __grid_consta
         if (edge && lim_min < len) {
             uint32_t nan = 0;
 #pragma unroll
-            for (int r = 0; r < 8; ++r)
+            for (int r = 0; r < 8; ++r) {
+                if (v_key(r) >= len - blk * 32) continue;
+                const auto look = [&](auto words, int d) {
+                    uint32_t x[decltype(words)::value];
+                    v_piece(st, r, d, x);
 #pragma unroll
-                for (int c = 0; c < S::VC; ++c) {
-                    if (v_key(r) >= len - blk * 32) continue;
+                    for (int w = 0; w < decltype(words)::value; ++w) nan |= ((x[w] & 0x7f7f7f7fu) + 0x01010101u) & 0x80808080u;
+                };
 #pragma unroll
-                    for (int w = 0; w < S::VB / 4; ++w)
-                        nan |= ((reinterpret_cast<const uint32_t*>(st + v_at(r, c))[w] & 0x7f7f7f7fu) + 0x01010101u) & 0x80808080u;
-                }
+                for (int c = 0; c < S::VC; ++c) look(std::integral_constant<int, S::VB / 4>(), S::VB * (g + 8 * c));
+                if constexpr (S::TAIL) look(std::integral_constant<int, 1>(), DP - 32 + 4 * g);
+            }
             if (__any_sync(0xffffffffu, nan != 0)) {
                 if constexpr (F32) {
 #pragma unroll
                     for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
-                        for (int j = 0; j < DP / 16; ++j)
+                        for (int j = 0; j < S::VT; ++j)
 #pragma unroll
                             for (int e = 0; e < 4; ++e) o[nt][j][e] *= fac[nt][e & 1] * vfac;
                 }
@@ -474,8 +484,8 @@ decode_q8_kernel(const __grid_constant__ CUtensorMap tmap_k, const __grid_consta
 #pragma unroll
                                 for (int x = 0; x < 2; ++x) w[x] = __shfl_sync(0xffffffffu, s[nt][mt][2 * y + x], i * 4 + t) * vw;
 #pragma unroll
-                                for (int j = 0; j < DP / 16; ++j) {
-                                    const int d = S::VB * (g + 8 * (j / (S::VB / 2))) + 2 * (j % (S::VB / 2));
+                                for (int j = 0; j < S::VT; ++j) {
+                                    const int d = S::v_channel(j, g);
                                     float f[4];
                                     q8::e4m3_values(d < p.D ? *reinterpret_cast<const uint16_t*>(row + d) : 0u, f);
 #pragma unroll
@@ -489,58 +499,53 @@ decode_q8_kernel(const __grid_constant__ CUtensorMap tmap_k, const __grid_consta
             }
         }
         // ---- values.  With f32 queries a block's sums start from zero and are added to O, scaled anew on the way, in f32.
+        // one piece of the channels of all 32 keys at a time
+        const int behind = len - blk * 32;
+        const auto tiles = [&](auto words, int j0, int d) {      // words of a key's piece, its first tile and channel
+            constexpr int W = decltype(words)::value;
+            uint32_t x[8][W];
 #pragma unroll
-        for (int c = 0; c < S::VC; ++c) {
-            constexpr int VW = S::VB / 4;
-            uint32_t x[2][4][VW];
+            for (int r = 0; r < 8; ++r) v_piece(st, r, d, x[r]);
+            if (behind < 32) {                                   // what lies behind the last key is nobody's, and may be NaN
 #pragma unroll
-            for (int mt = 0; mt < 2; ++mt)
+                for (int r = 0; r < 8; ++r)
+                    if (v_key(r) >= behind) {
 #pragma unroll
-                for (int r = 0; r < 4; ++r) {
-                    const uint8_t* src = st + v_at(4 * mt + r, c);
-                    if constexpr (VW == 4) *reinterpret_cast<uint4*>(x[mt][r]) = *reinterpret_cast<const uint4*>(src);
-                    else *reinterpret_cast<uint2*>(x[mt][r]) = *reinterpret_cast<const uint2*>(src);
-                }
-            if (blk * 32 + 32 > len) {                           // what lies behind the last key is nobody's, and may be NaN
-#pragma unroll
-                for (int mt = 0; mt < 2; ++mt)
-#pragma unroll
-                    for (int r = 0; r < 4; ++r)
-                        if (v_key(4 * mt + r) >= len - blk * 32) {
-#pragma unroll
-                            for (int w = 0; w < VW; ++w) x[mt][r][w] = 0;
-                        }
+                        for (int w = 0; w < W; ++w) x[r][w] = 0;
+                    }
             }
 #pragma unroll
-            for (int w = 0; w < VW; ++w)
+            for (int jj = 0; jj < 2 * W; ++jj) {
+                uint32_t a[2][4];
 #pragma unroll
-                for (int k = 0; k < 2; ++k) {
-                    const int j = c * (S::VB / 2) + 2 * w + k;               // channels VB (g + 8 c) + 4 w + 2 k and the next
-                    uint32_t a[2][4];
+                for (int h = 0; h < 2; ++h) {
+                    const uint32_t e0 = __byte_perm(x[4 * h][jj / 2], x[4 * h + 1][jj / 2], jj & 1 ? 0x7362 : 0x5140);
+                    const uint32_t e1 = __byte_perm(x[4 * h + 2][jj / 2], x[4 * h + 3][jj / 2], jj & 1 ? 0x7362 : 0x5140);
+                    a[h][0] = q8::e4m3_lo(e0); a[h][1] = q8::e4m3_hi(e0); a[h][2] = q8::e4m3_lo(e1); a[h][3] = q8::e4m3_hi(e1);
+                }
 #pragma unroll
-                    for (int mt = 0; mt < 2; ++mt) {
-                        const uint32_t e0 = __byte_perm(x[mt][0][w], x[mt][1][w], k ? 0x7362 : 0x5140), e1 = __byte_perm(x[mt][2][w], x[mt][3][w], k ? 0x7362 : 0x5140);
-                        a[mt][0] = q8::e4m3_lo(e0); a[mt][1] = q8::e4m3_hi(e0); a[mt][2] = q8::e4m3_lo(e1); a[mt][3] = q8::e4m3_hi(e1);
-                    }
+                for (int nt = 0; nt < NT; ++nt) {
+                    float (&to)[4] = o[nt][j0 + jj];
+                    if constexpr (F32) {
+                        float sum[4] = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
-                    for (int nt = 0; nt < NT; ++nt) {
-                        if constexpr (F32) {
-                            float sum[4] = {0.f, 0.f, 0.f, 0.f};
+                        for (int part = 1; part >= 0; --part)
 #pragma unroll
-                            for (int part = 1; part >= 0; --part)
+                            for (int h = 0; h < 2; ++h) mma16816(sum, a[h][0], a[h][1], a[h][2], a[h][3], pw[nt][h][part][0], pw[nt][h][part][1]);
 #pragma unroll
-                                for (int mt = 0; mt < 2; ++mt) mma16816(sum, a[mt][0], a[mt][1], a[mt][2], a[mt][3], pw[nt][mt][part][0], pw[nt][mt][part][1]);
+                        for (int e = 0; e < 4; ++e) to[e] = fmaf(to[e], fac[nt][e & 1] * vfac, sum[e]);
+                    } else {
 #pragma unroll
-                            for (int e = 0; e < 4; ++e) o[nt][j][e] = fmaf(o[nt][j][e], fac[nt][e & 1] * vfac, sum[e]);
-                        } else {
+                        for (int h = 0; h < 2; ++h)
 #pragma unroll
-                            for (int mt = 0; mt < 2; ++mt)
-#pragma unroll
-                                for (int part = 0; part < 2; ++part) mma16816(o[nt][j], a[mt][0], a[mt][1], a[mt][2], a[mt][3], pw[nt][mt][part][0], pw[nt][mt][part][1]);
-                        }
+                            for (int part = 0; part < 2; ++part) mma16816(to, a[h][0], a[h][1], a[h][2], a[h][3], pw[nt][h][part][0], pw[nt][h][part][1]);
                     }
                 }
-        }
+            }
+        };
+#pragma unroll
+        for (int c = 0; c < S::VC; ++c) tiles(std::integral_constant<int, S::VB / 4>(), c * (S::VB / 2), S::VB * (g + 8 * c));
+        if constexpr (S::TAIL) tiles(std::integral_constant<int, 1>(), S::VT - 2, DP - 32 + 4 * g);
         if (++stage == S::STAGES) { stage = 0; phase ^= 1u; }
     }
     if (MODE != DQ_EVEN || unit >= unit_end) chain_next();
@@ -560,8 +565,8 @@ decode_q8_kernel(const __grid_constant__ CUtensorMap tmap_k, const __grid_consta
 #pragma unroll
         for (int nt = 0; nt < NT; ++nt) {
 #pragma unroll
-            for (int j = 0; j < DP / 16; ++j) {
-                const int d = S::VB * (g + 8 * (j / (S::VB / 2))) + 2 * (j % (S::VB / 2));
+            for (int j = 0; j < S::VT; ++j) {
+                const int d = S::v_channel(j, g);
 #pragma unroll
                 for (int e = 0; e < 4; ++e) mine[(nt * 8 + 2 * t + (e & 1)) * S::OS + d + (e >> 1)] = o[nt][j][e] * down;
             }
@@ -659,9 +664,9 @@ decode_q8_kernel(const __grid_constant__ CUtensorMap tmap_k, const __grid_consta
 template <typename T>
 __global__ void __launch_bounds__(256) decode_q8_join_kernel(const DecodeQ8Params p, int tile_rows, int shares) {
     chain_wait();
-    __shared__ float s_w[DQ_MAX_BLOCKS], s_l[DQ_MAX_BLOCKS], s_r[16];
+    __shared__ float s_w[DQ_MAX_SHARES], s_l[DQ_MAX_SHARES], s_r[16];
     __shared__ __align__(16) float s_o[8][256];
-    __shared__ int s_at[DQ_MAX_BLOCKS];
+    __shared__ int s_at[DQ_MAX_SHARES];
     const int r = blockIdx.x, tile = blockIdx.z, Hkv = p.H / p.G, b = blockIdx.y / Hkv, kvh = blockIdx.y % Hkv;
     const int rr = tile * tile_rows + r, lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
     if (rr >= p.G * p.Tq) return;
@@ -740,22 +745,31 @@ __global__ void __launch_bounds__(256) decode_q8_join_kernel(const DecodeQ8Param
 struct DecodeQ8Plan { int dp, nt, tiles, mode, splits, shares; };   // splits: blocks of a cluster; shares: of all blocks
 
 // How the work is cut.  Sixteen query rows share a walk where there are more than eight (heads up to 128 wide: the registers hold their O).
+// The host knows how many keys a slice can hold, not how many it holds.  Caches of 16384 keys and more are walked in even shares: one long
+// sequence among short ones then keeps the whole device busy, for a second launch.  Measured with f16, D = 128 (lengths uniform from 0 / all full,
+// us; even shares against the best of 1, 2, 4 and 8 blocks a slice): 16 slices of 65536 keys 36 / 54 against 61 / 93, 64 of 16384 36 / 55 against
+// 43 / 58, 256 of 16384 107 / 182 against 104 / 180, 512 of 16384 210 / 346 against 197 / 361; but 16 of 16384 18 / 23 against 18 / 27,
+// 64 of 4096 25 / 24 against 16 / 19, 512 of 4096 95 / 97 against 61 / 109.  Shorter ones get as many blocks a slice as fill two of every SM.
 DecodeQ8Plan plan_decode_q8(const deers_decode_q8_desc* d) {
     DecodeQ8Plan p;
-    p.dp = d->cache.D <= 64 ? 64 : d->cache.D <= 128 ? 128 : 256;
+    p.dp = d->cache.D > 128 ? 256 : (d->cache.D + 31) / 32 * 32;
     const int R = d->H / d->cache.H * d->Tq;
     p.nt = R > 8 && p.dp <= 128 ? 2 : 1;
     p.tiles = (R + 8 * p.nt - 1) / (8 * p.nt);
     const long long slices = (long long)d->cache.B * d->cache.H * p.tiles;
     const long long blocks = (d->cache.capacity + 31) / 32;
-    long long want = (2 * 148 + slices - 1) / slices;
-    const long long most = (blocks + 7) / 8;                     // at least 256 keys a chunk
-    if (want > most) want = most;
-    if (want < 1) want = 1;
-    const char* e = getenv("DQMODE");
-    int mode = want == 1 ? DQ_SLICE : want <= 8 ? DQ_CLUSTER : DQ_EVEN, sp = (int)want, sh = 296;
-    if (e) sscanf(e, "%d,%d,%d", &mode, &sp, &sh);
-    p.mode = mode; p.splits = mode == DQ_CLUSTER ? sp : 1; p.shares = mode == DQ_EVEN ? sh : 0;
+    p.mode = DQ_SLICE; p.splits = 1; p.shares = 0;
+    if (d->cache.capacity >= DQ_LONG && d->cache.B <= DQ_MAX_EVEN) {
+        const long long most = slices * blocks / 14, fill = p.dp > 128 ? DQ_MAX_SHARES / 2 : DQ_MAX_SHARES;      // (heads of 256: one block of threads an SM)
+        p.mode = DQ_EVEN;
+        p.shares = (int)(most < fill ? most : fill);
+    } else {
+        long long want = DQ_MAX_SHARES / slices;
+        const long long most = (blocks + 7) / 8;                 // at least 256 keys a chunk
+        if (want > most) want = most;
+        if (want > 8) want = 8;
+        if (want > 1) { p.mode = DQ_CLUSTER; p.splits = (int)want; }
+    }
     return p;
 }
 
@@ -820,8 +834,13 @@ int decode_q8_launch(deers_ctx* ctx, const DecodeQ8Params& p, const DecodeQ8Plan
 
 template <typename T>
 int decode_q8_widths(deers_ctx* ctx, const DecodeQ8Params& p, const DecodeQ8Plan& plan, int slices, const deers_cache_q8& c) {
-    if (plan.dp == 64) return plan.nt == 2 ? decode_q8_launch<T, 64, 2>(ctx, p, plan, slices, c) : decode_q8_launch<T, 64, 1>(ctx, p, plan, slices, c);
-    if (plan.dp == 128) return plan.nt == 2 ? decode_q8_launch<T, 128, 2>(ctx, p, plan, slices, c) : decode_q8_launch<T, 128, 1>(ctx, p, plan, slices, c);
+    switch (plan.dp) {
+        case 32: return plan.nt == 2 ? decode_q8_launch<T, 32, 2>(ctx, p, plan, slices, c) : decode_q8_launch<T, 32, 1>(ctx, p, plan, slices, c);
+        case 64: return plan.nt == 2 ? decode_q8_launch<T, 64, 2>(ctx, p, plan, slices, c) : decode_q8_launch<T, 64, 1>(ctx, p, plan, slices, c);
+        case 96: return plan.nt == 2 ? decode_q8_launch<T, 96, 2>(ctx, p, plan, slices, c) : decode_q8_launch<T, 96, 1>(ctx, p, plan, slices, c);
+        case 128: return plan.nt == 2 ? decode_q8_launch<T, 128, 2>(ctx, p, plan, slices, c) : decode_q8_launch<T, 128, 1>(ctx, p, plan, slices, c);
+        default: break;
+    }
     return decode_q8_launch<T, 256, 1>(ctx, p, plan, slices, c);
 }
 

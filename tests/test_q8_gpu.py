@@ -336,7 +336,10 @@ DECODE = [  # B, H, G, Tq, D, cap, lengths
     (1, 1, 1, 1, 16, 1, [1]), (1, 12, 1, 1, 64, 800, [777]), (2, 4, 2, 1, 32, 100, [0, 100]), (3, 6, 3, 2, 80, 300, [1, 2, 299]),
     (2, 8, 8, 1, 128, 513, [512, 33]), (2, 16, 8, 2, 96, 400, [400, 31]), (1, 8, 4, 5, 256, 130, [130]), (2, 3, 1, 7, 48, 64, [3, 64]),
     (1, 2, 1, 1, 64, 20000, [19999]), (1, 1, 1, 3, 128, 40000, [39000]), (5, 2, 2, 8, 112, 257, [5, 8, 100, 256, 257]), (1, 32, 32, 2, 64, 600, [555]),
-    (40, 8, 1, 1, 128, 96, list(range(57, 97)))]
+    (40, 8, 1, 1, 128, 96, list(range(57, 97))), (1, 4, 4, 3, 32, 90, [77]), (2, 2, 1, 1, 96, 500, [311, 500]), (20, 16, 1, 1, 64, 40, list(range(1, 41, 2))),
+    # (caches from 16384 keys on are walked in even shares of all sequences' keys)
+    (3, 8, 4, 3, 96, 17000, [0, 17000, 5]), (2, 4, 4, 1, 256, 16384, [16384, 7]), (40, 1, 1, 1, 16, 16384, [(i * i * 37) % 1700 for i in range(39)] + [16384]),
+    (3, 2, 2, 8, 32, 16385, [16385, 9, 16384]), (2, 2, 2, 2, 64, 16400, [0, 0])]
 
 
 @TYPES
@@ -368,8 +371,8 @@ def test_decode_of_views_and_token_major_queries(dtype):
 
 
 @TYPES
-@pytest.mark.parametrize("D,cap,splits", [(64, 90, 1), (128, 700, 8), (256, 5000, 9)])
-def test_decode_is_not_reached_by_what_it_does_not_see(D, cap, splits, dtype):
+@pytest.mark.parametrize("D,cap", [(64, 90), (128, 700), (256, 5000), (96, 17000), (32, 75)])
+def test_decode_is_not_reached_by_what_it_does_not_see(D, cap, dtype):
     """NaN codes behind the last row, and in keys that some of a call's rows see and others do not."""
     g = gen(D)
     k, ks, v, vs = filled(g, 2, 2, cap, D)
