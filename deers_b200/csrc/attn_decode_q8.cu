@@ -31,8 +31,8 @@ int deers_check_cache(const deers_cache_q8* c);
 namespace {
 
 constexpr int DQ_WARPS = 4;
-constexpr int DQ_MAX_SHARES = 2 * 148, DQ_MAX_EVEN = 256;        // even shares: blocks of threads and sequences at most
-constexpr int DQ_LONG = 16384;                                   // keys a slice can hold from which on shares are even
+constexpr int DQ_MAX_SHARES = 2 * 148, DQ_MAX_EVEN = 64;         // even shares: blocks of threads and slices at most
+constexpr int DQ_LONG = 16384;                                   // keys of a long slice
 constexpr float DQ_LOG2E = 1.4426950408889634f, DQ_LN2 = 0.6931471805599453f;
 constexpr float DQ_UP = 32768.0f;                                // weights are at most 2^15 of f16's 65504
 
@@ -189,6 +189,7 @@ decode_q8_kernel(const __grid_constant__ CUtensorMap tmap_k, const __grid_consta
     for (bool first = true; MODE == DQ_EVEN ? unit < unit_end : first; first = false) {
     int b, kvh, tile, len, blk0, blk1;
     bool whole = true;                                           // this block of threads sees all keys of the slice
+    int chunks = 1;                                              // DQ_CLUSTER: blocks of threads that share them
     if constexpr (MODE == DQ_EVEN) {
         int lo = 0, hi = p.B;                                    // the last sequence that begins at or before the unit
         while (hi - lo > 1) {
@@ -233,7 +234,14 @@ decode_q8_kernel(const __grid_constant__ CUtensorMap tmap_k, const __grid_consta
     if constexpr (MODE != DQ_EVEN) {
         len = length(b);
         const int blocks = (len + 31) / 32, split = MODE == DQ_CLUSTER ? blockIdx.x : 0;
-        blk0 = (int)((long long)blocks * split / p.splits); blk1 = (int)((long long)blocks * (split + 1) / p.splits);
+        if constexpr (MODE == DQ_CLUSTER) {
+            // chunks have 256 keys or more: the cluster's other blocks leave (its barrier waits for those that stay; all have come to the first)
+            chunks = max(1, min(p.splits, (blocks + 7) / 8));
+            whole = chunks == 1;
+            if (split >= chunks || whole) cooperative_groups::this_cluster().barrier_wait();
+            if (split >= chunks) return;
+        }
+        blk0 = (int)((long long)blocks * split / chunks); blk1 = (int)((long long)blocks * (split + 1) / chunks);
     }
     const uint8_t* vb = p.v + b * p.sv[0] + kvh * p.sv[1];
     const float* ksl = p.k_scale + b * p.skl[0] + kvh * p.skl[1];
@@ -596,8 +604,8 @@ decode_q8_kernel(const __grid_constant__ CUtensorMap tmap_k, const __grid_consta
     };
     // (a share begins inside at most one slice, and ends inside at most one)
     float* to_part = MODE == DQ_EVEN ? p.part + ((long long)blockIdx.x * 2 + (blk0 > 0 ? 0 : 1)) * (S::ROWS * (p.D + 4)) : nullptr;
-    const int share = ((rows * p.D + p.splits - 1) / p.splits + 3) / 4 * 4;             // DQ_CLUSTER: of the outputs, to every block
-    if constexpr (MODE == DQ_CLUSTER) cooperative_groups::this_cluster().barrier_wait();       // (all have started: their memory may be written to)
+    const int share = ((rows * p.D + chunks - 1) / chunks + 3) / 4 * 4;             // DQ_CLUSTER: of the outputs, to every block
+    if (MODE == DQ_CLUSTER && !whole) cooperative_groups::this_cluster().barrier_wait();       // (all have started: their memory may be written to)
     for (int r = warp; r < rows; r += DQ_WARPS) {
         float w[DQ_WARPS], mx = -INFINITY, sum = 0.f;
 #pragma unroll
@@ -615,7 +623,7 @@ decode_q8_kernel(const __grid_constant__ CUtensorMap tmap_k, const __grid_consta
             float4 v = make_float4(0.f, 0.f, 0.f, 0.f);
 #pragma unroll
             for (int x = 0; x < DQ_WARPS; ++x) add4(v, w[x], *reinterpret_cast<const float4*>(&meet[(x * S::ROWS + r) * S::OS + d]));
-            if constexpr (MODE == DQ_CLUSTER) {
+            if (MODE == DQ_CLUSTER && !whole) {
                 const int i = r * p.D + d, z = i / share;
                 const uint32_t to = sm100::cluster_addr(smem + S::SENT, z);
                 send4(to + 8 * 8 * S::ROWS + 4 * (blockIdx.x * share + i - z * share), v);
@@ -632,7 +640,7 @@ decode_q8_kernel(const __grid_constant__ CUtensorMap tmap_k, const __grid_consta
             }
         }
     }
-    if constexpr (MODE == DQ_CLUSTER) {
+    if (MODE == DQ_CLUSTER && !whole) {
         cooperative_groups::this_cluster().sync();
         const float2* ml = reinterpret_cast<const float2*>(smem + S::SENT);
         const float* parts = reinterpret_cast<const float*>(ml + 8 * S::ROWS);
@@ -643,13 +651,13 @@ decode_q8_kernel(const __grid_constant__ CUtensorMap tmap_k, const __grid_consta
             float4 v = make_float4(0.f, 0.f, 0.f, 0.f);
 #pragma unroll
             for (int z = 0; z < 8; ++z) {
-                w[z] = z < p.splits ? ml[z * S::ROWS + r].x : -INFINITY;
+                w[z] = z < chunks ? ml[z * S::ROWS + r].x : -INFINITY;
                 mx = fmaxf(mx, w[z]);
             }
             const float ms = mx == -INFINITY ? 0.f : mx;
 #pragma unroll
             for (int z = 0; z < 8; ++z)
-                if (z < p.splits) {
+                if (z < chunks) {
                     const float f = exp2f(w[z] - ms);
                     sum = fmaf(f, ml[z * S::ROWS + r].y, sum);
                     add4(v, f, *reinterpret_cast<const float4*>(&parts[z * share + j]));
@@ -745,11 +753,13 @@ __global__ void __launch_bounds__(256) decode_q8_join_kernel(const DecodeQ8Param
 struct DecodeQ8Plan { int dp, nt, tiles, mode, splits, shares; };   // splits: blocks of a cluster; shares: of all blocks
 
 // How the work is cut.  Sixteen query rows share a walk where there are more than eight (heads up to 128 wide: the registers hold their O).
-// The host knows how many keys a slice can hold, not how many it holds.  Caches of 16384 keys and more are walked in even shares: one long
-// sequence among short ones then keeps the whole device busy, for a second launch.  Measured with f16, D = 128 (lengths uniform from 0 / all full,
-// us; even shares against the best of 1, 2, 4 and 8 blocks a slice): 16 slices of 65536 keys 36 / 54 against 61 / 93, 64 of 16384 36 / 55 against
-// 43 / 58, 256 of 16384 107 / 182 against 104 / 180, 512 of 16384 210 / 346 against 197 / 361; but 16 of 16384 18 / 23 against 18 / 27,
-// 64 of 4096 25 / 24 against 16 / 19, 512 of 4096 95 / 97 against 61 / 109.  Shorter ones get as many blocks a slice as fill two of every SM.
+// The host knows how many keys a slice can hold, not how many it holds.  Each slice gets as many blocks of threads (a cluster, 8 at most) as put
+// two on every SM, or seven where slices are long: ragged lengths then leave less of the device idle at the end (512 slices of 16384 keys, lengths
+// uniform from 0 / all full: 2 blocks 188 / 350 us, 1 block 225 / 472);
+// those whose lengths leave them less than 256 keys go again at once.  Few long slices are cut into even shares of all keys instead, for a second
+// launch (f16, D = 128, even shares against 8 blocks a slice): 16 slices of 65536 keys 36 / 54 us against 61 / 93, 64 of 16384 36 / 55 against
+// 43 / 67, 16 of 16384 18 / 23 against 18 / 27; but 64 of 4096 25 / 24 against 17 / 24 (16 / 19 of 4 blocks), and where such caches hold a few keys
+// only, 32 slices of up to 500 keys 14 against 7, 512 of them 48 against 14: many slices are never cut so.
 DecodeQ8Plan plan_decode_q8(const deers_decode_q8_desc* d) {
     DecodeQ8Plan p;
     p.dp = d->cache.D > 128 ? 256 : (d->cache.D + 31) / 32 * 32;
@@ -759,12 +769,12 @@ DecodeQ8Plan plan_decode_q8(const deers_decode_q8_desc* d) {
     const long long slices = (long long)d->cache.B * d->cache.H * p.tiles;
     const long long blocks = (d->cache.capacity + 31) / 32;
     p.mode = DQ_SLICE; p.splits = 1; p.shares = 0;
-    if (d->cache.capacity >= DQ_LONG && d->cache.B <= DQ_MAX_EVEN) {
+    if (d->cache.capacity >= DQ_LONG && slices <= DQ_MAX_EVEN) {
         const long long most = slices * blocks / 14, fill = p.dp > 128 ? DQ_MAX_SHARES / 2 : DQ_MAX_SHARES;      // (heads of 256: one block of threads an SM)
         p.mode = DQ_EVEN;
         p.shares = (int)(most < fill ? most : fill);
     } else {
-        long long want = DQ_MAX_SHARES / slices;
+        long long want = (d->cache.capacity >= DQ_LONG ? 7 * 148 : 2 * 148) / slices;
         const long long most = (blocks + 7) / 8;                 // at least 256 keys a chunk
         if (want > most) want = most;
         if (want > 8) want = 8;

@@ -167,4 +167,4 @@ def test_attn_decode_q8_refuses():
     for strides in ((0, 1280, 32), (3840, 0, 32)):               # a cache that several sequences or heads share
         assert call(d(cache(k_strides=(ctypes.c_int64 * 3)(*strides)))) == _lib.ERR_LAYOUT
     size = lambda **c: L.deers_b200_attn_decode_q8_workspace_bytes(d(cache(**c), H=2))  # noqa: E731
-    assert size(B=256, H=1, capacity=16384) > 0 and size(B=257, H=1, capacity=16384) == 0 and size(B=1, H=1, capacity=16383) == 0
+    assert size(B=64, H=1, capacity=16384) > 0 and size(B=65, H=1, capacity=16384) == 0 and size(B=1, H=1, capacity=16383) == 0

@@ -337,9 +337,9 @@ DECODE = [  # B, H, G, Tq, D, cap, lengths
     (2, 8, 8, 1, 128, 513, [512, 33]), (2, 16, 8, 2, 96, 400, [400, 31]), (1, 8, 4, 5, 256, 130, [130]), (2, 3, 1, 7, 48, 64, [3, 64]),
     (1, 2, 1, 1, 64, 20000, [19999]), (1, 1, 1, 3, 128, 40000, [39000]), (5, 2, 2, 8, 112, 257, [5, 8, 100, 256, 257]), (1, 32, 32, 2, 64, 600, [555]),
     (40, 8, 1, 1, 128, 96, list(range(57, 97))), (1, 4, 4, 3, 32, 90, [77]), (2, 2, 1, 1, 96, 500, [311, 500]), (20, 16, 1, 1, 64, 40, list(range(1, 41, 2))),
-    # (caches from 16384 keys on are walked in even shares of all sequences' keys)
+    # (up to 64 slices of 16384 keys and more are walked in even shares of all keys)
     (3, 8, 4, 3, 96, 17000, [0, 17000, 5]), (2, 4, 4, 1, 256, 16384, [16384, 7]), (40, 1, 1, 1, 16, 16384, [(i * i * 37) % 1700 for i in range(39)] + [16384]),
-    (3, 2, 2, 8, 32, 16385, [16385, 9, 16384]), (2, 2, 2, 2, 64, 16400, [0, 0])]
+    (3, 2, 2, 8, 32, 16385, [16385, 9, 16384]), (2, 2, 2, 2, 64, 16400, [0, 0]), (65, 2, 2, 1, 16, 16384, [(i * i * 37) % 1700 for i in range(64)] + [16384])]
 
 
 @TYPES
