@@ -108,6 +108,9 @@ struct Shape {
     // (the ring has been read when the warps meet; what other blocks of a cluster send has a place of its own)
     static constexpr int SENT = RING > MERGE ? RING : MERGE, BARS = SENT + 8 * ROWS * 8 + PART + 8 * 32;
     static constexpr int SMEM = BARS + DQ_WARPS * STAGES * 8 + 16;                 // (DQ_EVEN: and the sequences' blocks)
+    // Blocks of threads on an SM: what shared memory has place for, or two where sixteen rows' registers count (with q in shared memory instead three
+    // go on, and are slower: 39 -> 44 us for 37 x 8 slices of 2048 keys of 128, G 16, f16).
+    static constexpr int ON_AN_SM = DP == 256 ? 1 : NT == 2 && DP >= 96 ? 2 : 3;
     // first of the four channels of product step i, of the two channels of tile j (a tile's rows 8 to 15 are the next ones)
     static __device__ __forceinline__ int k_channel(int i, int t) { return i < 4 * KC ? 16 * (t + 4 * (i / 4)) + 4 * (i % 4) : DP - 32 + 8 * t + 4 * (i - 4 * KC); }
     static __device__ __forceinline__ int v_channel(int j, int g) {
@@ -143,7 +146,7 @@ __device__ __forceinline__ void decode_q8_prologue(const void* tmap_k, const voi
 }
 
 template <typename T, int DP, int NT, int MODE>
-__global__ void __launch_bounds__(32 * DQ_WARPS)
+__global__ void __launch_bounds__(32 * DQ_WARPS, Shape<DP, NT>::ON_AN_SM)
 decode_q8_kernel(const __grid_constant__ CUtensorMap tmap_k, const __grid_constant__ CUtensorMap tmap_v, const DecodeQ8Params p) {
     decode_q8_prologue<DP, NT>(&tmap_k, &tmap_v);
     chain_wait();
