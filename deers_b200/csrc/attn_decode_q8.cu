@@ -40,8 +40,7 @@ struct DecodeQ8Params {
     const void* q; void* o; float* lse;
     const uint8_t* k; const uint8_t* v; const float* k_scale; const float* v_scale;
     const int* lengths;
-    long long* before;                                           // DQ_EVEN: [B + 1] blocks of all slices of the sequences before
-    float* part;                                                 // [block of threads][2][rows of a tile][D + 4]: O, maximum, sum
+    float* part;                                                 // DQ_EVEN: [block of threads][rows of a tile][D + 4]: O, maximum, sum
     long long sq[3], so[3], sk[3], sv[3], skl[2], svl[2];
     int B, H, G, Tq, D, cap, causal, splits, tiles, q_vec, o_vec;
     float scale;
@@ -107,7 +106,7 @@ struct Shape {
     static constexpr int PART = ROWS * DP * 4;                   // DQ_CLUSTER: [block][its share of O] and, before, [block][row] maximum and sum
     // (the ring has been read when the warps meet; what other blocks of a cluster send has a place of its own)
     static constexpr int SENT = RING > MERGE ? RING : MERGE, BARS = SENT + 8 * ROWS * 8 + PART + 8 * 32;
-    static constexpr int SMEM = BARS + DQ_WARPS * STAGES * 8 + 16;                 // (DQ_EVEN: and the sequences' blocks)
+    static constexpr int SMEM = BARS + DQ_WARPS * STAGES * 8 + 16;
     // Blocks of threads on an SM: what shared memory has place for, or two where sixteen rows' registers count (with q in shared memory instead three
     // go on, and are slower: 39 -> 44 us for 37 x 8 slices of 2048 keys of 128, G 16, f16).
     static constexpr int ON_AN_SM = DP == 256 ? 1 : NT == 2 && DP >= 96 ? 2 : 3;
@@ -122,12 +121,42 @@ struct Shape {
 // all blocks of all slices, whatever their lengths.
 enum DecodeQ8Mode { DQ_SLICE = 0, DQ_CLUSTER = 1, DQ_EVEN = 2 };
 
-// n even shares of all units: share i starts at all * i / n.
-struct Shares {
-    long long each;
-    int rest, n;
-    __device__ __forceinline__ Shares(long long all, int n_) : each(all / n_), rest((int)(all % n_)), n(n_) {}
-    __device__ __forceinline__ long long start(int i) const { return each * i + (unsigned)(rest * i) / (unsigned)n; }
+// DQ_EVEN: every slice is cut into chunks of at most `unit` blocks of keys, all of one size or one block apart, in the order of the slices; unit is
+// the least for which `shares` blocks of threads are enough whatever the lengths.  Every warp works it out, two sequences a lane.
+struct Cuts {
+    int len[2], n[2], end[2];                                    // keys; chunks of each of its slices; chunks of all slices up to its last
+    template <typename F>
+    __device__ __forceinline__ Cuts(int B, int slices_each, int shares, F length) {
+        const int lane = threadIdx.x & 31;
+        int all = 0;
+#pragma unroll
+        for (int i = 0; i < 2; ++i) {
+            len[i] = lane + 32 * i < B ? length(lane + 32 * i) : 0;
+            all += (len[i] + 31) / 32;
+        }
+#pragma unroll
+        for (int off = 16; off >= 1; off >>= 1) all += __shfl_xor_sync(0xffffffffu, all, off);
+        const int rest = shares - B * slices_each, unit = max(1, (all * slices_each + rest - 1) / rest);
+        int before = 0;
+#pragma unroll
+        for (int i = 0; i < 2; ++i) {
+            n[i] = ((len[i] + 31) / 32 + unit - 1) / unit;
+            end[i] = n[i] * slices_each;
+#pragma unroll
+            for (int off = 1; off < 32; off *= 2) {
+                const int up = __shfl_up_sync(0xffffffffu, end[i], off);
+                if (lane >= off) end[i] += up;
+            }
+            end[i] += before;
+            before = __shfl_sync(0xffffffffu, end[i], 31);
+        }
+    }
+    // sequence of chunk c (B or more: there is none)
+    __device__ __forceinline__ int sequence(int c) const {
+        const int b = __popc(__ballot_sync(0xffffffffu, end[0] <= c)), more = __popc(__ballot_sync(0xffffffffu, end[1] <= c));
+        return b < 32 ? b : 32 + more;
+    }
+    static __device__ __forceinline__ int of(const int (&x)[2], int b) { return __shfl_sync(0xffffffffu, b < 32 ? x[0] : x[1], b & 31); }
 };
 
 // Barriers: nothing of global memory.
@@ -161,54 +190,22 @@ decode_q8_kernel(const __grid_constant__ CUtensorMap tmap_k, const __grid_consta
         if (len < 0 || len > p.cap) atomicCAS(p.err, 0u, (unsigned)DEERS_KERR_CACHE | 2u);
         return min(max(len, 0), p.cap);
     };
-    long long* before = reinterpret_cast<long long*>(smem + S::SMEM);
-    long long unit = 0, unit_end = 0;                            // DQ_EVEN: this block's, of all slices' blocks in a row
-    if constexpr (MODE == DQ_EVEN) {
-        if (warp == 0) {
-            long long run = 0;
-            for (int b0 = 0; b0 < p.B; b0 += 32) {
-                long long n = b0 + lane < p.B ? (long long)((length(b0 + lane) + 31) / 32) * Hkv * p.tiles : 0;
-#pragma unroll
-                for (int off = 1; off < 32; off *= 2) {
-                    const long long up = __shfl_up_sync(0xffffffffu, n, off);
-                    if (lane >= off) n += up;
-                }
-                if (b0 + lane < p.B) before[b0 + lane + 1] = run + n;
-                run += __shfl_sync(0xffffffffu, n, 31);
-            }
-            if (lane == 0) before[0] = 0;
-            __syncwarp();
-            if (blockIdx.x == 0)
-                for (int i = lane; i <= p.B; i += 32) p.before[i] = before[i];
-        }
-        __syncthreads();
-        const Shares shares(before[p.B], gridDim.x);
-        unit = shares.start(blockIdx.x);
-        unit_end = shares.start(blockIdx.x + 1);
-    }
     if constexpr (MODE == DQ_CLUSTER) cooperative_groups::this_cluster().barrier_arrive();
     int stage = 0;                                               // of this warp's ring: where its next block is
     uint32_t phase = 0;
-    for (bool first = true; MODE == DQ_EVEN ? unit < unit_end : first; first = false) {
     int b, kvh, tile, len, blk0, blk1;
     bool whole = true;                                           // this block of threads sees all keys of the slice
     int chunks = 1;                                              // DQ_CLUSTER: blocks of threads that share them
     if constexpr (MODE == DQ_EVEN) {
-        int lo = 0, hi = p.B;                                    // the last sequence that begins at or before the unit
-        while (hi - lo > 1) {
-            const int mid = (lo + hi) / 2;
-            if (before[mid] <= unit) lo = mid;
-            else hi = mid;
-        }
-        b = lo;
-        const long long rest = unit - before[b], blocks = (before[b + 1] - before[b]) / (Hkv * p.tiles);
-        const int slice = (int)(rest / blocks);
+        const Cuts cuts(p.B, Hkv * p.tiles, gridDim.x, length);
+        b = cuts.sequence(blockIdx.x);
+        if (b >= p.B) return;
+        len = Cuts::of(cuts.len, b);
+        const int n = Cuts::of(cuts.n, b), c = n * Hkv * p.tiles - (Cuts::of(cuts.end, b) - (int)blockIdx.x), slice = c / n, blocks = (len + 31) / 32;
         kvh = slice / p.tiles; tile = slice % p.tiles;
-        len = min(max(p.lengths[b], 0), p.cap);
-        blk0 = (int)(rest % blocks);
-        blk1 = (int)min(blocks, blk0 + (unit_end - unit));
-        whole = blk0 == 0 && blk1 == (int)blocks;
-        unit += blk1 - blk0;
+        blk0 = blocks * (c % n) / n;
+        blk1 = blocks * (c % n + 1) / n;
+        whole = n == 1;
     } else {
         b = blockIdx.y / Hkv; kvh = blockIdx.y % Hkv; tile = blockIdx.z;
     }
@@ -252,13 +249,7 @@ decode_q8_kernel(const __grid_constant__ CUtensorMap tmap_k, const __grid_consta
 
     uint64_t* full = reinterpret_cast<uint64_t*>(smem + S::BARS) + warp * S::STAGES;
     const sm100::WaitState ws{reinterpret_cast<uint32_t*>(smem + S::BARS + DQ_WARPS * S::STAGES * 8), p.err};
-    if (MODE == DQ_EVEN) sm100::fence_proxy_async_smem();        // (the ring has been written by threads)
-    // the barriers are there, and the ring is free
-    if (MODE == DQ_EVEN && !first) {
-        if (__syncthreads_or(*ws.abort != 0)) break;
-    } else {
-        __syncthreads();
-    }
+    __syncthreads();                                             // the barriers are there
     uint8_t* ring = smem + warp * (S::STAGES * S::STAGE_BYTES);
     // Block `blk` into stage s, by one lane.  (Keys behind the sequence's last may lie in it, and are masked below.)
     auto fetch = [&](int blk, int s) {
@@ -559,7 +550,7 @@ decode_q8_kernel(const __grid_constant__ CUtensorMap tmap_k, const __grid_consta
         if constexpr (S::TAIL) tiles(std::integral_constant<int, 1>(), S::VT - 2, DP - 32 + 4 * g);
         if (++stage == S::STAGES) { stage = 0; phase ^= 1u; }
     }
-    if (MODE != DQ_EVEN || unit >= unit_end) chain_next();
+    chain_next();
 
     // ---- the warps meet
 #pragma unroll
@@ -605,8 +596,7 @@ decode_q8_kernel(const __grid_constant__ CUtensorMap tmap_k, const __grid_consta
         put4(out_row(r) + d, make_float4(v.x * inv, v.y * inv, v.z * inv, v.w * inv), p.o_vec);
         if (p.lse && d == 0) *lse_at(r) = (mx + log2f(sum)) * DQ_LN2;
     };
-    // (a share begins inside at most one slice, and ends inside at most one)
-    float* to_part = MODE == DQ_EVEN ? p.part + ((long long)blockIdx.x * 2 + (blk0 > 0 ? 0 : 1)) * (S::ROWS * (p.D + 4)) : nullptr;
+    float* to_part = p.part + (long long)blockIdx.x * (S::ROWS * (p.D + 4));      // DQ_EVEN
     const int share = ((rows * p.D + chunks - 1) / chunks + 3) / 4 * 4;             // DQ_CLUSTER: of the outputs, to every block
     if (MODE == DQ_CLUSTER && !whole) cooperative_groups::this_cluster().barrier_wait();       // (all have started: their memory may be written to)
     for (int r = warp; r < rows; r += DQ_WARPS) {
@@ -668,7 +658,6 @@ decode_q8_kernel(const __grid_constant__ CUtensorMap tmap_k, const __grid_consta
             finish(r, i - r * p.D, v, mx, sum);
         }
     }
-    }
 }
 
 // Rows of slices that no block of threads has seen whole, from what each has left of them; one row a block.
@@ -677,41 +666,33 @@ __global__ void __launch_bounds__(256) decode_q8_join_kernel(const DecodeQ8Param
     chain_wait();
     __shared__ float s_w[DQ_MAX_SHARES], s_l[DQ_MAX_SHARES], s_r[16];
     __shared__ __align__(16) float s_o[8][256];
-    __shared__ int s_at[DQ_MAX_SHARES];
     const int r = blockIdx.x, tile = blockIdx.z, Hkv = p.H / p.G, b = blockIdx.y / Hkv, kvh = blockIdx.y % Hkv;
     const int rr = tile * tile_rows + r, lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
     if (rr >= p.G * p.Tq) return;
-    const long long all = p.before[p.B], here = p.before[b], blocks = (p.before[b + 1] - here) / (Hkv * p.tiles);
-    const long long u0 = here + (kvh * p.tiles + tile) * blocks, u1 = u0 + blocks;
+    const Cuts cuts(p.B, Hkv * p.tiles, shares, [&](int x) { return min(max(p.lengths[x], 0), p.cap); });
+    const int n = Cuts::of(cuts.n, b), first = Cuts::of(cuts.end, b) - n * (Hkv * p.tiles - kvh * p.tiles - tile);
+    if (n == 1) return;                                          // seen whole
     const int head = kvh * p.G + rr / p.Tq, i = rr % p.Tq;
     T* o = static_cast<T*>(p.o) + b * p.so[0] + head * p.so[1] + i * p.so[2];
     float* lse = p.lse ? p.lse + ((long long)b * p.H + head) * p.Tq + i : nullptr;
-    if (blocks == 0) {                                           // a sequence without keys is nobody's share
+    if (n == 0) {                                                // a sequence without keys is nobody's share
         for (int d = threadIdx.x; d < p.D; d += 256) put(o + d, 0.f);
         if (lse && threadIdx.x == 0) *lse = -INFINITY;
         return;
     }
-    const Shares sh(all, shares);
-    const auto share_of = [&](long long u) {                     // the share that unit u is in: the last one that starts at or before it
-        int c = (int)(u * shares / all);
-        while (c + 1 < shares && sh.start(c + 1) <= u) ++c;
-        while (sh.start(c) > u) --c;
-        return c;
-    };
-    const int c0 = share_of(u0), n = share_of(u1 - 1) - c0 + 1;
-    if (n == 1) return;                                          // seen whole
     const int step = tile_rows * (p.D + 4);
-    const float* part = p.part + r * (p.D + 4);
+    const float* part = p.part + (long long)first * step + r * (p.D + 4);
     float mx = -INFINITY;
     for (int z = threadIdx.x; z < n; z += 256) {
-        // (the first share has it as its end, or from its own start; the others begin inside; a share of nothing has left nothing)
-        const long long from = sh.start(c0 + z);
-        const int at = sh.start(c0 + z + 1) > from ? (c0 + z) * 2 + (from > u0 ? 0 : 1) : -1;
-        s_at[z] = at;
-        const float2 ms = at < 0 ? make_float2(-INFINITY, 0.f) : *reinterpret_cast<const float2*>(part + (long long)at * step + p.D);
+        const float2 ms = *reinterpret_cast<const float2*>(part + z * step + p.D);
         s_w[z] = ms.x; s_l[z] = ms.y;
         mx = fmaxf(mx, ms.x);
     }
+    // (what the first turn below wants is on its way meanwhile)
+    float4 early[4];
+#pragma unroll
+    for (int i = 0; i < 4; ++i)
+        early[i] = warp + 8 * i < n && 4 * lane < p.D ? *reinterpret_cast<const float4*>(part + (warp + 8 * i) * step + 4 * lane) : make_float4(0.f, 0.f, 0.f, 0.f);
 #pragma unroll
     for (int off = 16; off >= 1; off >>= 1) mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, off));
     if (lane == 0) s_r[warp] = mx;
@@ -721,7 +702,7 @@ __global__ void __launch_bounds__(256) decode_q8_join_kernel(const DecodeQ8Param
     const float ms = mx == -INFINITY ? 0.f : mx;
     float sum = 0.f;
     for (int z = threadIdx.x; z < n; z += 256) {
-        const float w = s_at[z] < 0 ? 0.f : exp2f(s_w[z] - ms);
+        const float w = exp2f(s_w[z] - ms);
         s_w[z] = w;
         sum = fmaf(w, s_l[z], sum);
     }
@@ -732,15 +713,17 @@ __global__ void __launch_bounds__(256) decode_q8_join_kernel(const DecodeQ8Param
     sum = 0.f;
 #pragma unroll
     for (int w = 0; w < 8; ++w) sum += s_r[8 + w];
-    // a warp adds up every eighth share, four channels a lane
+    // a warp adds up every eighth chunk, four channels a lane
     for (int d = 4 * lane; d < p.D; d += 128) {
         float4 v = make_float4(0.f, 0.f, 0.f, 0.f);
-#pragma unroll 8
-        for (int z = warp; z < n; z += 8) {
-            const float w = s_w[z];
-            const float4 x = s_at[z] < 0 ? make_float4(0.f, 0.f, 0.f, 0.f) : *reinterpret_cast<const float4*>(part + (long long)s_at[z] * step + d);
-            add4(v, w, x);
+        int z = warp;
+        if (d < 128) {
+#pragma unroll
+            for (int i = 0; i < 4; ++i, z += 8)
+                if (z < n) add4(v, s_w[z], early[i]);
         }
+#pragma unroll 4
+        for (; z < n; z += 8) add4(v, s_w[z], *reinterpret_cast<const float4*>(part + z * step + d));
         *reinterpret_cast<float4*>(&s_o[warp][d]) = v;
     }
     __syncthreads();
@@ -786,10 +769,9 @@ DecodeQ8Plan plan_decode_q8(const deers_decode_q8_desc* d) {
     return p;
 }
 
-size_t decode_q8_head(const deers_decode_q8_desc* d) { return ((size_t)(d->cache.B + 1) * sizeof(long long) + 255) / 256 * 256; }
 size_t decode_q8_bytes(const deers_decode_q8_desc* d, const DecodeQ8Plan& p) {
     if (p.mode != DQ_EVEN) return 0;
-    return decode_q8_head(d) + (size_t)p.shares * 2 * (8 * p.nt) * (d->cache.D + 4) * sizeof(float);
+    return (size_t)p.shares * (8 * p.nt) * (d->cache.D + 4) * sizeof(float);
 }
 
 int decode_q8_check(const deers_decode_q8_desc* d) {
@@ -836,9 +818,8 @@ int decode_q8_launch(deers_ctx* ctx, const DecodeQ8Params& p, const DecodeQ8Plan
         DEERS_SMEM_ONCE(ctx, (decode_q8_kernel<T, DP, NT, DQ_CLUSTER>), S::SMEM);
         DEERS_CUDA_TRY(ctx, launch_chained(ctx, decode_q8_kernel<T, DP, NT, DQ_CLUSTER>, dim3(plan.splits, slices, plan.tiles), 32 * DQ_WARPS, S::SMEM, plan.splits, tk, tv, p));
     } else {
-        const int smem = S::SMEM + (p.B + 1) * (int)sizeof(long long);
-        DEERS_SMEM_ONCE(ctx, (decode_q8_kernel<T, DP, NT, DQ_EVEN>), S::SMEM + (DQ_MAX_EVEN + 1) * sizeof(long long));
-        DEERS_CUDA_TRY(ctx, launch_chained(ctx, decode_q8_kernel<T, DP, NT, DQ_EVEN>, (unsigned)plan.shares, 32 * DQ_WARPS, smem, 1, tk, tv, p));
+        DEERS_SMEM_ONCE(ctx, (decode_q8_kernel<T, DP, NT, DQ_EVEN>), S::SMEM);
+        DEERS_CUDA_TRY(ctx, launch_chained(ctx, decode_q8_kernel<T, DP, NT, DQ_EVEN>, (unsigned)plan.shares, 32 * DQ_WARPS, S::SMEM, 1, tk, tv, p));
         DEERS_CUDA_TRY(ctx, launch_chained(ctx, decode_q8_join_kernel<T>, dim3(S::ROWS, slices, plan.tiles), 256, 0, 1, p, S::ROWS, plan.shares));
         ctx->launches += 1;
     }
@@ -878,7 +859,7 @@ extern "C" int deers_b200_attn_decode_q8(deers_ctx* ctx, const deers_decode_q8_d
     const deers_cache_q8& c = d->cache;
     DecodeQ8Params p;
     p.q = q; p.o = o; p.lse = lse; p.lengths = lengths;
-    p.before = (long long*)workspace; p.part = need ? (float*)((char*)workspace + decode_q8_head(d)) : nullptr;
+    p.part = need ? (float*)workspace : nullptr;
     p.k = (const uint8_t*)c.k; p.v = (const uint8_t*)c.v; p.k_scale = c.k_scale; p.v_scale = c.v_scale;
     for (int i = 0; i < 3; ++i) { p.sq[i] = d->q_strides[i]; p.so[i] = d->o_strides[i]; p.sk[i] = c.k_strides[i]; p.sv[i] = c.v_strides[i]; }
     for (int i = 0; i < 2; ++i) { p.skl[i] = c.k_scale_strides[i]; p.svl[i] = c.v_scale_strides[i]; }
