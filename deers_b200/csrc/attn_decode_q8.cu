@@ -740,12 +740,11 @@ struct DecodeQ8Plan { int dp, nt, tiles, mode, splits, shares; };   // splits: b
 
 // How the work is cut.  Sixteen query rows share a walk where there are more than eight (heads up to 128 wide: the registers hold their O).
 // The host knows how many keys a slice can hold, not how many it holds.  Each slice gets as many blocks of threads (a cluster, 8 at most) as put
-// two on every SM, or seven where slices are long: ragged lengths then leave less of the device idle at the end (512 slices of 16384 keys, lengths
-// uniform from 0 / all full: 2 blocks 188 / 350 us, 1 block 225 / 472);
-// those whose lengths leave them less than 256 keys go again at once.  Few long slices are cut into even shares of all keys instead, for a second
-// launch (f16, D = 128, even shares against 8 blocks a slice): 16 slices of 65536 keys 36 / 54 us against 61 / 93, 64 of 16384 36 / 55 against
-// 43 / 67, 16 of 16384 18 / 23 against 18 / 27; but 64 of 4096 25 / 24 against 17 / 24 (16 / 19 of 4 blocks), and where such caches hold a few keys
-// only, 32 slices of up to 500 keys 14 against 7, 512 of them 48 against 14: many slices are never cut so.
+// two on every SM, or seven where slices are long: ragged lengths then leave less of the device idle at the end (512 slices of 16384 keys, f16,
+// D = 128, lengths uniform from 0 / all full: 2 blocks 188 / 350 us, 1 block 225 / 472).  Blocks whose lengths leave them less than 256 keys go
+// again at once.  Few long slices are cut on the device in proportion to their keys, for a second launch (against 8 blocks a slice): 16 slices of
+// 65536 keys 31 / 49 us against 61 / 93, 64 of 16384 33 / 52 against 43 / 67, 16 of 16384 13 / 20 against 18 / 27.  Shorter ones gain nothing
+// (32 of 8192 keys 15 / 20 against 15 / 19; 32 of 4096 13 / 15 against 12 / 14).
 DecodeQ8Plan plan_decode_q8(const deers_decode_q8_desc* d) {
     DecodeQ8Plan p;
     p.dp = d->cache.D > 128 ? 256 : (d->cache.D + 31) / 32 * 32;
