@@ -303,7 +303,7 @@ decode_q8_kernel(const __grid_constant__ CUtensorMap tmap_k, const __grid_consta
             top = max(top, __shfl_xor_sync(0xffffffffu, top, 2));
             // a power of two that brings the largest value to 2^14 .. 2^15 (exponents of factor and inverse both in range)
             int e = 141 - (int)(top >> 23);
-            e = top == 0 || top >= 0x7f800000u ? 0 : max(-100, min(100, e));
+            e = top == 0 || top >= 0x7f800000u ? 0 : min(100, e);       // (-113 or more)
             up = __uint_as_float((unsigned)(127 + e) << 23);
             back = __uint_as_float((unsigned)(127 - e) << 23);
         }
@@ -563,14 +563,13 @@ decode_q8_kernel(const __grid_constant__ CUtensorMap tmap_k, const __grid_consta
     float* meet = reinterpret_cast<float*>(smem);
     {
         float* mine = meet + warp * S::ROWS * S::OS;
-        const float down = vref * (1.0f / DQ_UP);
 #pragma unroll
         for (int nt = 0; nt < NT; ++nt) {
 #pragma unroll
             for (int j = 0; j < S::VT; ++j) {
                 const int d = S::v_channel(j, g);
 #pragma unroll
-                for (int e = 0; e < 4; ++e) mine[(nt * 8 + 2 * t + (e & 1)) * S::OS + d + (e >> 1)] = o[nt][j][e] * down;
+                for (int e = 0; e < 4; ++e) mine[(nt * 8 + 2 * t + (e & 1)) * S::OS + d + (e >> 1)] = o[nt][j][e] * (1.0f / DQ_UP) * vref;      // (vref / 2^15 may be a subnormal)
             }
             if (g == 0) {
 #pragma unroll

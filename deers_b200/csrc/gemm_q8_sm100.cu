@@ -566,7 +566,7 @@ extern "C" int deers_b200_gemm_q8(deers_ctx* ctx, int32_t M, int32_t N, int32_t 
     if (code != DEERS_I8 && code != DEERS_E4M3) return DEERS_ERR_DTYPE;
     if (out_dtype != DEERS_F16 && out_dtype != DEERS_F32) return DEERS_ERR_DTYPE;
     if (M < 0 || N < 1 || K < 1) return DEERS_ERR_SHAPE;
-    if (code == DEERS_I8 && K > 131072) return DEERS_ERR_UNSUPPORTED;        // 2^31 / 128^2: sums stay whole numbers of 32 bits
+    if (code == DEERS_I8 && K >= 131072) return DEERS_ERR_UNSUPPORTED;       // 2^31 / 128^2: sums stay whole numbers of 32 bits
     if (M == 0) return DEERS_OK;
     if (!a || !b || !c || !a_scale || !b_scale) return DEERS_ERR_NULL;
     const uintptr_t es = out_dtype == DEERS_F16 ? 2 : 4;

@@ -225,6 +225,7 @@ extern "C" int deers_b200_quantize_rows(deers_ctx* ctx, const deers_quantize_des
     if (d->dtype != DEERS_F16 && d->dtype != DEERS_F32) return DEERS_ERR_DTYPE;
     if (d->code != DEERS_I8 && d->code != DEERS_E4M3) return DEERS_ERR_DTYPE;
     if (d->rows < 0 || d->rows > 0x7fffffffLL || d->C < 1) return DEERS_ERR_SHAPE;
+    if (d->C > (1 << 30)) return DEERS_ERR_UNSUPPORTED;          // (places behind a row's end stay within 31 bits)
     if (d->relu_squared && (d->norm || residual || sum)) return DEERS_ERR_UNSUPPORTED;
     if (d->rows == 0) return DEERS_OK;
     if (!x || !codes || !scale || (residual && !sum)) return DEERS_ERR_NULL;

@@ -100,7 +100,7 @@ def quantize_weight_q8(weight, dtype: torch.dtype = torch.int8) -> RowsQ8:
 
 def linear_q8(rows: RowsQ8, weight: RowsQ8, out_dtype: torch.dtype = torch.float16) -> torch.Tensor:
     """``x.matmul(weight)`` of ``Linear::forward`` (src/nn.rs:184-190) on codes: [.., in_features] times a weight of ``quantize_weight_q8``
-    (codes of the same type) to [.., out_features], f16 or f32, rounded once.  int8 sums are exact (in_features <= 131072), e4m3 sums f32."""
+    (codes of the same type) to [.., out_features], f16 or f32, rounded once.  int8 sums are exact (in_features < 131072), e4m3 sums f32."""
     if out_dtype not in _DTYPES:
         raise DTypeMismatch(f"linear_q8: f16 or f32 comes out, got {out_dtype}")
     out = _DTYPES[out_dtype]
@@ -209,7 +209,9 @@ def _places(name: str, t: torch.Tensor, of: torch.Tensor) -> torch.Tensor:
 def attention_decode_q8(q, cache: CacheQ8, lengths: torch.Tensor, scale: Optional[float] = None, causal: bool = True, want_lse: bool = False):
     """``attention_decode`` over a cache of codes: q [B, Hq, Tq, D] (f16 or f32; Hq a multiple of the cache's heads, head h reads head
     ``h // (Hq / H)``), ``lengths[b]`` rows of sequence b, the Tq newest of which belong to the queries.  Returns o [B, Hq, Tq, D] (and lse
-    [B, Hq, Tq]).  A row that sees no key has o = 0 and lse = -inf; what lies behind a sequence's last row is not read."""
+    [B, Hq, Tq]).  A row that sees no key has o = 0 and lse = -inf; what lies behind a sequence's last row is not read.  Of a batch padded at
+    the back to T rows the lengths are ``start + T``: query t then sees rows up to its own, and what the padding's queries see is nobody's.
+    Lengths beyond the capacity are taken as the capacity, and ``Context.sync`` reports them."""
     if scale is None and q.dim() == 4:
         scale = default_scale(q.shape[3])
     held = (cache.k, cache.v, cache.k_scale, cache.v_scale)

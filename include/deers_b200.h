@@ -458,7 +458,7 @@ int deers_b200_cross_entropy_bwd(deers_ctx* ctx, int64_t rows, int64_t vocab, co
  */
 typedef struct deers_quantize_desc {
     int64_t rows;
-    int32_t C;
+    int32_t C;                /* at most 2^30 */
     int32_t dtype;            /* of x, residual and sum: DEERS_F16 / DEERS_F32 */
     int32_t code;             /* DEERS_I8 / DEERS_E4M3 */
     int32_t norm, relu_squared;
@@ -470,7 +470,7 @@ int deers_b200_quantize_rows(deers_ctx* ctx, const deers_quantize_desc* desc, co
 
 /*
  * c[m, n] = a_scale[m] * b_scale[n] * sum_k a[m, k] b[n, k]: rows of codes times a weight laid out [out_features, in_features], both K
- * contiguous and of one code type.  int8 sums are exact (K <= 131072); e4m3 sums are f32.  c is rounded once, to out_dtype (DEERS_F16 / DEERS_F32).
+ * contiguous and of one code type.  int8 sums are exact (K < 131072); e4m3 sums are f32.  c is rounded once, to out_dtype (DEERS_F16 / DEERS_F32).
  * a, b: 16-byte aligned, lda and ldb multiples of 16; c: any leading dimension (16-byte stores where rows allow).
  */
 int deers_b200_gemm_q8(deers_ctx* ctx, int32_t M, int32_t N, int32_t K, int32_t code, const void* a, int64_t lda, const float* a_scale,

@@ -80,6 +80,7 @@ def test_quantize_rows_refuses():
     assert f(CTX, desc(rows=0), None, None, None, None, None) == _lib.OK
     for bad in (dict(rows=-1), dict(C=0), dict(rows=1 << 31)):
         assert f(CTX, desc(**bad), P, None, None, P, P) == _lib.ERR_SHAPE
+    assert f(CTX, desc(C=(1 << 30) + 1, ld_codes=(1 << 30) + 16), P, None, None, P, P) == _lib.ERR_UNSUPPORTED
     for bad in (dict(dtype=2), dict(code=0)):
         assert f(CTX, desc(**bad), P, None, None, P, P) == _lib.ERR_DTYPE
     assert f(CTX, desc(relu_squared=1), P, None, None, P, P) == _lib.ERR_UNSUPPORTED
@@ -101,7 +102,8 @@ def test_gemm_q8_refuses():
         assert call(**bad) == _lib.ERR_SHAPE
     for bad in (dict(code=_lib.F16), dict(out=_lib.I8)):
         assert call(**bad) == _lib.ERR_DTYPE
-    assert call(K=131073, lda=1 << 18, ldb=1 << 18) == _lib.ERR_UNSUPPORTED
+    for K in (131072, 131073):                                   # 131072 products of -128 and -128 leave 32 bits
+        assert call(K=K, lda=1 << 18, ldb=1 << 18) == _lib.ERR_UNSUPPORTED
     for bad in (dict(lda=31), dict(lda=16), dict(ldb=40), dict(ldc=7), dict(a=P + 8), dict(b=P + 1), dict(c=P + 1), dict(sa=P + 2), dict(sb=P + 1)):
         assert call(**bad) == _lib.ERR_LAYOUT
 

@@ -223,6 +223,13 @@ def test_linear_with_the_largest_codes_and_scales_of_no_number():
     check_linear(a, sa, b, sb, E4M3)
 
 
+def test_linear_with_the_longest_sums_of_whole_numbers():
+    # 131071 products of -128 and -128, the last that fit 32 bits (quantised rows have no -128, a caller's may)
+    a, b = torch.full((2, 131071), -128.0).double(), torch.full((3, 131071), -128.0).double()
+    a[1] = 127.0
+    check_linear(a, torch.tensor([1e-3, 1.0]), b, torch.tensor([1e-4, 1e-5, 1.0]), I8, torch.float32)
+
+
 # ---- the cache ----------------------------------------------------------------------------------------------------------
 def cache_values(c):
     return c.k.float().cpu().double(), c.k_scale.cpu(), c.v.float().cpu().double(), c.v_scale.cpu()
@@ -417,6 +424,15 @@ def test_decode_with_scales_of_all_sizes():
         check_decode(torch.randn(1, 2, 1, 64, generator=g) * f, (k, ks, v, vs), torch.tensor([256], dtype=torch.int32), scale=0.1 / f if f > 1e-20 else 1.0)
 
 
+def test_decode_of_the_smallest_and_largest_numbers():
+    """f32: values next to the subnormals keep their bits, queries beyond f16's largest times 2^100 are scaled into its range."""
+    g = gen(43)
+    n = torch.tensor([250], dtype=torch.int32)
+    k, ks, v, vs = filled(g, 1, 2, 256, 64)
+    check_decode(torch.zeros(1, 2, 1, 64), (k, ks, v, vs * 1e-35), n)        # (equal weights: nothing but the values' own error)
+    check_decode(torch.randn(1, 2, 1, 64, generator=g) * 1e36, (k, ks, v, vs), n, scale=1e-37)
+
+
 def test_decode_of_lengths_outside_of_the_cache_is_told():
     from deers_b200.errors import CudaError
     g = gen(51)
@@ -491,6 +507,26 @@ def test_a_block_decodes_step_by_step(codes):
             assert off < (0.1 if codes is E4M3 else 0.05), off
         at += T
     sync()
+
+
+def test_a_padded_batch_of_prompts():
+    """Prompts of unlike lengths, padded at the back: query t of every sequence sees rows up to its own when the lengths are start + T; what the
+    padding's queries see is nobody's."""
+    g = gen(67)
+    B, H, T, D = 3, 2, 45, 64
+    counts = torch.tensor([45, 1, 33], dtype=torch.int32)
+    k, v = (torch.randn(B, H, T, D, generator=g).half() for _ in range(2))
+    q = torch.randn(B, 2 * H, T, D, generator=g).half()
+    cache = q8().CacheQ8.new(B, H, 64, D)
+    start = torch.tensor([0, 16, 2], dtype=torch.int32)
+    cache.append(k.cuda(), v.cuda(), start.cuda(), counts.cuda())
+    got = q8().attention_decode_q8(q.cuda(), cache, (start + T).cuda(), want_lse=True)
+    sync()
+    values = cache_values(cache)
+    for i in range(B):
+        n = int(counts[i])
+        one = [t[i:i + 1] for t in values]
+        check_decode(q[i:i + 1, :, :n], (one[0], one[1], one[2], one[3]), start[i:i + 1] + n, got=[t[i:i + 1, :, :n] for t in got])
 
 
 def test_a_captured_step_serves_every_length():
