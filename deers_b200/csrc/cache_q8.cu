@@ -6,7 +6,8 @@
 // other rows and blocks stay as they are.  So one scale serves a block however its rows arrive, a block that starts anew forgets what lay
 // there, and writing the same rows again changes nothing.  A value that is no number is stored as NaN and takes no part in the scale.
 // A group of threads (a warp, or four) owns a block of one head of keys or values: it reads the new rows once, into registers.
-// Bound: HBM, 3 bytes an element with f16; for single tokens the launch.
+// Bound: HBM, 3 bytes an element with f16 (8 x 8 heads of 2048 rows of 256 33.8 us, 5.2 TB/s; f32 46.4, 6.3), instructions below 256 channels (of 128 20.0 us,
+// 4.4 TB/s; f32 24.3, 6.0); for single tokens the launch.  Values next to a border between codes are decided last: f16 24 -> 21 us, f32 27 -> 24.
 #include "common.cuh"
 #include "q8_codes.cuh"
 
@@ -27,9 +28,11 @@ __device__ __forceinline__ float as_f(float v) { return v; }
 __device__ __forceinline__ __half not_a_number(__half) { return __ushort_as_half(0x7e00); }
 __device__ __forceinline__ float not_a_number(float) { return __uint_as_float(0x7fc00000u); }
 
-// 32 * NW threads own a token block, LR threads a row of it, eight values each; NP rows of a thread stay in registers.
+// 32 * NW threads own a token block, LR threads a row of it, eight values each; NP rows of a thread stay in registers.  Whole blocks of f16 hide
+// their loads behind other blocks: ten on an SM for heads up to 64 (14.2 -> 13.2 us for 8 x 8 heads of 2048 rows), eight up to 128 (20.7 -> 20.0);
+// wider ones have 64 values a thread, and are quicker with the registers that they ask for (39.3 -> 33.8).
 template <typename T, bool VEC, int LR, int NW, int NP>
-__global__ void __launch_bounds__(128) append_q8_kernel(const AppendParams p) {
+__global__ void __launch_bounds__(128, NW == 4 && sizeof(T) == 2 ? (LR == 8 ? 10 : LR == 16 ? 8 : 1) : 1) append_q8_kernel(const AppendParams p) {
     chain_begin();
     constexpr int NT = 32 * NW, PER = 128 / NT, STEP = NT / LR;  // groups of a block of threads; rows at a time
     const int tid = threadIdx.x % NT, warp = threadIdx.x / 32;
@@ -69,14 +72,7 @@ __global__ void __launch_bounds__(128) append_q8_kernel(const AppendParams p) {
         float top = 0.f;
 #pragma unroll
         for (int i = 0; i < NP; ++i) {
-            if (i * STEP < rows) {
-#pragma unroll
-                for (int e = 0; e < 8; e += 4) {
-                    float f[4];
-                    q8::four(v[i] + e, f);
-                    q8::look_at(top, f);
-                }
-            }
+            if (i * STEP < rows) q8::look_at8(top, v[i]);
         }
 #pragma unroll
         for (int off = 16; off >= 1; off >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, off));
@@ -106,6 +102,37 @@ __global__ void __launch_bounds__(128) append_q8_kernel(const AppendParams p) {
     const bool grown = fresh > was;
     const float scale = grown ? fresh : was;
     if (tid == 0) *scale_at = scale;
+    const float den = scale > 0.f ? scale : 1.0f;
+    const q8::Factors factors = q8::factors(1.0f, den, q8::den_is_far(den));
+    uint8_t* to = codes + (lo + row) * p.sc[kv][2] + col;
+    uint32_t near = 0;                                           // groups of four values that hold one next to a border
+#pragma unroll
+    for (int i = 0; i < NP; ++i) {
+        if (i * STEP < rows) {
+            uint32_t c[2];
+#pragma unroll
+            for (int k = 0; k < 2; ++k) {
+                float f[4];
+                uint32_t up;
+                q8::four(v[i] + 4 * k, f);
+                q8::bounds_e4m3(f, factors, c[k], up);
+                if (c[k] != up) near |= 1u << (2 * i + k);
+            }
+            *reinterpret_cast<uint2*>(to + i * STEP * p.sc[kv][2]) = make_uint2(c[0], c[1]);
+        }
+    }
+    // They are decided behind everything else, from memory again: a call where the rows' registers live costs more than its own time.
+#pragma unroll 1
+    for (; near; near &= near - 1) {
+        const int j = __ffs((int)near) - 1, i = j >> 1, k = j & 1;
+        float f[4];
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+            f[e] = as_f(src[i * STEP * p.ss[kv][2] + 4 * k + e]);
+            if (fabsf(f[e]) == inf) f[e] = __uint_as_float(0x7fc00000u);
+        }
+        *reinterpret_cast<uint32_t*>(to + i * STEP * p.sc[kv][2] + 4 * k) = q8::quotients_e4m3(f[0], f[1], f[2], f[3], 1.0f, den);
+    }
     if (grown && begin > first) {                                // the earlier rows, 16 bytes at a time
         const q8::Factors again = q8::factors(was, scale, q8::den_is_far(scale) || !(was > 1e-20f));
         const int per16 = p.D / 16, old16 = (begin - first) * per16;
@@ -121,22 +148,6 @@ __global__ void __launch_bounds__(128) append_q8_kernel(const AppendParams p) {
                 out[k] = q8::codes_of<false>(f, again, was, scale);
             }
             *c = make_uint4(out[0], out[1], out[2], out[3]);
-        }
-    }
-    const float den = scale > 0.f ? scale : 1.0f;
-    const q8::Factors factors = q8::factors(1.0f, den, q8::den_is_far(den));
-    uint8_t* to = codes + (lo + row) * p.sc[kv][2] + col;
-#pragma unroll
-    for (int i = 0; i < NP; ++i) {
-        if (i * STEP < rows) {
-            uint32_t c[2];
-#pragma unroll
-            for (int k = 0; k < 2; ++k) {
-                float f[4];
-                q8::four(v[i] + 4 * k, f);
-                c[k] = q8::codes_of<false>(f, factors, 1.0f, den);
-            }
-            *reinterpret_cast<uint2*>(to + i * STEP * p.sc[kv][2]) = make_uint2(c[0], c[1]);
         }
     }
 }

@@ -101,16 +101,43 @@ static __device__ __noinline__ uint32_t decide_i8(float v0, float v1, float v2, 
     return w;
 }
 
-// Codes of four quotients v[i] * num / den, each the nearest code to the exact quotient (ties to even).  Where both bounds of a quotient have one
-// code, that is it; the few others are decided exactly, so the codes follow from the operator's definition alone, not from the order of this
-// kernel's operations.  (f16 values meet borders often: three normal ones in ten thousand.)
-template <bool I8>
-__device__ __forceinline__ uint32_t codes_of(const float (&v)[4], const Factors& f, float num, float den) {
-    const uint64_t v01 = pack_f32x2(v[0], v[1]), v23 = pack_f32x2(v[2], v[3]), up = pack_f32x2(f.up, f.up);
-    float u[4];
+// e4m3 codes of four quotients v[i] * num / den whose numerators are f32 values.  A quotient within its last bit leaves a remainder that is an f32 value too,
+// and the remainder's sign says on which side of it the exact one lies: cut off, the last bit set where something was, it rounds as the exact one does.
+static __device__ __noinline__ uint32_t quotients_e4m3(float v0, float v1, float v2, float v3, float num, float den) {
+    if (den_is_far(den)) return codes_far<false>(v0, v1, v2, v3, num, den);
+    const float v[4] = {v0, v1, v2, v3}, r = 1.0f / den;
+    float t[4];
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+        const float x = v[i] * num, near = x * r, q = fmaf(fmaf(-near, den, x), r, near), rest = fmaf(-q, den, x);
+        const uint32_t bits = __float_as_uint(q);
+        t[i] = __uint_as_float(rest != 0.f ? (bits - ((bits ^ __float_as_uint(rest)) >> 31)) | 1u : bits);
+    }
+    return e4m3_of(t[0], t[1], t[2], t[3]);
+}
+
+// Codes of both bounds of four quotients: one where they are equal.
+__device__ __forceinline__ void bounds_e4m3(const float (&v)[4], const Factors& f, uint32_t& lo, uint32_t& hi) {
+    const uint64_t v01 = pack_f32x2(v[0], v[1]), v23 = pack_f32x2(v[2], v[3]), up = pack_f32x2(f.up, f.up), down = pack_f32x2(f.down, f.down);
+    float u[4], d[4];
     unpack_f32x2(mul2(v01, up), u[0], u[1]);
     unpack_f32x2(mul2(v23, up), u[2], u[3]);
+    unpack_f32x2(mul2(v01, down), d[0], d[1]);
+    unpack_f32x2(mul2(v23, down), d[2], d[3]);
+    lo = e4m3_of(d[0], d[1], d[2], d[3]);
+    hi = e4m3_of(u[0], u[1], u[2], u[3]);
+}
+
+// Codes of four quotients v[i] * num / den, each the nearest code to the exact quotient (ties to even).  Where both bounds of a quotient have one
+// code, that is it; the few others are decided exactly, so the codes follow from the operator's definition alone, not from the order of this
+// kernel's operations.  (f16 values meet borders often: three normal ones in ten thousand, and a warp asks for 128 at once.)  EXACT: v[i] * num are f32 values,
+// which makes the decision short (norm of 16384 x 2048 f16 42.0 -> 41.3 us).
+template <bool I8, bool EXACT = false>
+__device__ __forceinline__ uint32_t codes_of(const float (&v)[4], const Factors& f, float num, float den) {
     if constexpr (I8) {
+        float u[4];
+        unpack_f32x2(mul2(pack_f32x2(v[0], v[1]), pack_f32x2(f.up, f.up)), u[0], u[1]);
+        unpack_f32x2(mul2(pack_f32x2(v[2], v[3]), pack_f32x2(f.up, f.up)), u[2], u[3]);
         constexpr float MAGIC = 12582912.0f;                      // 1.5 * 2^23: the sum's low bits are the nearest whole number
         uint32_t c[4];
         bool near = false;                                       // (of 127 the factor is off by 2^-14.6 at most: borders are looked for 2^-13 to either side)
@@ -123,12 +150,11 @@ __device__ __forceinline__ uint32_t codes_of(const float (&v)[4], const Factors&
         if (near) return decide_i8(v[0], v[1], v[2], v[3], num, den);
         return __byte_perm(__byte_perm(c[0], c[1], 0x0040), __byte_perm(c[2], c[3], 0x0040), 0x5410);
     } else {
-        const uint64_t down = pack_f32x2(f.down, f.down);
-        float d[4];
-        unpack_f32x2(mul2(v01, down), d[0], d[1]);
-        unpack_f32x2(mul2(v23, down), d[2], d[3]);
-        const uint32_t lo = e4m3_of(d[0], d[1], d[2], d[3]), hi = e4m3_of(u[0], u[1], u[2], u[3]);
-        return lo == hi ? lo : decide_e4m3(lo, hi, v[0], v[1], v[2], v[3], num, den);
+        uint32_t lo, hi;
+        bounds_e4m3(v, f, lo, hi);
+        if (lo == hi) return lo;
+        if constexpr (EXACT) return quotients_e4m3(v[0], v[1], v[2], v[3], num, den);
+        else return decide_e4m3(lo, hi, v[0], v[1], v[2], v[3], num, den);
     }
 }
 
@@ -141,6 +167,18 @@ __device__ __forceinline__ void four(const float* v, float (&f)[4]) {
 __device__ __forceinline__ void four(const __half* v, float (&f)[4]) {
     const float2 a = __half22float2(__halves2half2(v[0], v[1])), b = __half22float2(__halves2half2(v[2], v[3]));
     f[0] = a.x; f[1] = a.y; f[2] = b.x; f[3] = b.y;
+}
+// |v| of eight values into a running maximum that passes over NaN.
+__device__ __forceinline__ void look_at8(float& top, const float* v) {
+#pragma unroll
+    for (int e = 0; e < 8; e += 4) look_at(top, *reinterpret_cast<const float(*)[4]>(v + e));
+}
+__device__ __forceinline__ void look_at8(float& top, const __half* v) {
+    __half2 m = __habs2(__halves2half2(v[0], v[1]));
+#pragma unroll
+    for (int e = 2; e < 8; e += 2) m = __hmax2(m, __habs2(__halves2half2(v[e], v[e + 1])));
+    const float2 f = __half22float2(m);
+    top = fmaxf(top, fmaxf(f.x, f.y));
 }
 
 }  // namespace q8

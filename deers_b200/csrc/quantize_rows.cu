@@ -11,7 +11,7 @@
 // Bound: HBM, 7 bytes an element with f16 and a residual, 13 with f32: 16384 x 2048 f16 41 us (5.7 TB/s, 0.88 of the copy rate), 8192 x 4096 f32 79 us (0.85).
 // What it took: a row on as few threads as hold it in 40 registers, so that an SM has 1536 (48 -> 42 us; at 60 registers loads of too few rows
 // were in flight); borders between codes decided by exact products instead of a 64-bit division for every value next to one (relative to
-// that 51 -> 48, and new keys and values, cache_q8.cu, 141 -> 43); units that neighbouring threads interleave where rows start on no 16-byte
+// that 51 -> 48, and new keys and values, cache_q8.cu, 141 -> 43, by remainders of f16 quotients 42.0 -> 41.3); units that neighbouring threads interleave where rows start on no 16-byte
 // boundary (4096 x 4100 f16 106 -> 39 us).
 #include "common.cuh"
 #include "q8_codes.cuh"
@@ -169,7 +169,7 @@ __global__ void __launch_bounds__(TPR == 32 ? 256 : TPR, NP > 0 ? 1536 / (TPR ==
         for (int e = 0; e < N; e += 4) {
             float f[4];
             values(v, e, f);
-            c[e / 4] = some ? q8::codes_of<I8>(f, factors, MOST, top) : 0u;
+            c[e / 4] = some ? q8::codes_of<I8, sizeof(T) == 2 && !RELU2>(f, factors, MOST, top) : 0u;      // (448 has three bits, an f16 value eleven)
         }
 #pragma unroll
         for (int u = 0; u < UNITS; ++u) {

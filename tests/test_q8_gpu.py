@@ -297,6 +297,28 @@ def test_append_of_no_numbers_and_zeros():
     sync()
 
 
+@TYPES
+def test_append_of_values_at_borders_between_codes(dtype):
+    """Quotients on borders between codes and next to them, at scales that are powers of two and at others, tiny ones among them; and the earlier
+    rows of a block, rounded again to a scale that brings codes onto borders."""
+    every = torch.arange(127, dtype=torch.uint8).view(E4M3).double()
+    mid = (every[1:] + every[:-1]) / 2
+    x = torch.cat([mid, -mid, torch.tensor([448.0, 0.0, -0.0, 448.0])])          # 256
+    for f in (1.0, 2.0 ** -7, 0.7, 3.3) + ((1e-22, 1e25) if dtype is torch.float32 else ()):
+        t = (x * f).to(dtype)
+        rows = torch.stack([t, torch.nextafter(t, torch.full_like(t, math.inf)), torch.nextafter(t, torch.full_like(t, -math.inf))])[None, None]
+        c = q8().CacheQ8.new(1, 1, 40, 256)
+        k, ks, v, vs = cache_values(c)
+        for new, at in ((rows, 0), (rows * 2, 3), (rows * 3, 30)):
+            start = torch.tensor([at], dtype=torch.int32)
+            c.append(new.cuda(), new.flip(-1).cuda(), start.cuda())
+            ref.append(k, ks, new, start, [3])
+            ref.append(v, vs, new.flip(-1), start, [3])
+            for got, want in zip(cache_values(c), (k, ks, v, vs)):
+                same(got, want)
+    sync()
+
+
 def test_append_outside_of_the_cache_is_left_out_and_told():
     from deers_b200 import _lib
     from deers_b200.errors import CudaError
