@@ -45,6 +45,7 @@ struct DecodeQ8Params {
     int B, H, G, Tq, D, cap, causal, splits, tiles, q_vec, o_vec;
     float scale;
     unsigned int* err;
+    unsigned int* told;                                          // of lengths outside of the cache
 };
 
 __device__ __forceinline__ uint32_t pack2(float lo, float hi) {
@@ -187,7 +188,7 @@ decode_q8_kernel(const __grid_constant__ CUtensorMap tmap_k, const __grid_consta
     const int Hkv = p.H / p.G, R = p.G * p.Tq;
     const auto length = [&](int b) {
         const int len = p.lengths[b];
-        if (len < 0 || len > p.cap) atomicCAS(p.err, 0u, (unsigned)DEERS_KERR_CACHE | 2u);
+        if (len < 0 || len > p.cap) atomicCAS(p.told, 0u, (unsigned)DEERS_KERR_CACHE | 2u);
         return min(max(len, 0), p.cap);
     };
     if constexpr (MODE == DQ_CLUSTER) cooperative_groups::this_cluster().barrier_arrive();
@@ -863,7 +864,7 @@ extern "C" int deers_b200_attn_decode_q8(deers_ctx* ctx, const deers_decode_q8_d
     for (int i = 0; i < 2; ++i) { p.skl[i] = c.k_scale_strides[i]; p.svl[i] = c.v_scale_strides[i]; }
     p.B = c.B; p.tiles = plan.tiles;
     p.H = d->H; p.G = d->H / c.H; p.Tq = d->Tq; p.D = c.D; p.cap = c.capacity; p.causal = d->causal; p.splits = plan.splits;
-    p.scale = d->scale; p.err = ctx->dev_err;
+    p.scale = d->scale; p.err = ctx->dev_err; p.told = ctx->dev_err + 1;
     const int64_t al = 16 / (int64_t)es - 1;
     p.o_vec = ((uintptr_t)o & 15u) == 0 && ((d->o_strides[0] | d->o_strides[1] | d->o_strides[2]) & al) == 0;
     p.q_vec = ((uintptr_t)q & 15u) == 0 && ((d->q_strides[0] | d->q_strides[1] | d->q_strides[2]) & al) == 0;

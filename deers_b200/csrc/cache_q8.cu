@@ -20,7 +20,7 @@ struct AppendParams {
     long long ss[2][3], sc[2][3], sl[2][2];   // strides (b, h, t) in elements, of the scales (b, h)
     const int* start; const int* count;       // count may be nullptr: T rows of every sequence
     int H, T, D, cap;
-    unsigned int* err;
+    unsigned int* told;
 };
 
 __device__ __forceinline__ float as_f(__half v) { return __half2float(v); }
@@ -40,7 +40,7 @@ __global__ void __launch_bounds__(128, NW == 4 && sizeof(T) == 2 ? (LR == 8 ? 10
     const bool mine = h < p.H;                                   // (with NW == 4 the whole block)
     int begin = p.start[b], n = p.count ? p.count[b] : p.T;
     if (begin < 0 || n < 0 || n > p.T || (long long)begin + n > p.cap) {      // rows outside of the cache are left out, and told
-        if (threadIdx.x == 0 && blockIdx.x == 0) atomicCAS(p.err, 0u, (unsigned)DEERS_KERR_CACHE | 1u);
+        if (threadIdx.x == 0 && blockIdx.x == 0) atomicCAS(p.told, 0u, (unsigned)DEERS_KERR_CACHE | 1u);
         n = min(max(n, 0), p.T);
         if (begin < 0 || begin >= p.cap) n = 0;
         n = min(n, p.cap - begin);
@@ -215,7 +215,7 @@ extern "C" int deers_b200_cache_q8_append(deers_ctx* ctx, const deers_cache_q8* 
     p.codes[0] = (uint8_t*)c->k; p.codes[1] = (uint8_t*)c->v;
     p.scale[0] = c->k_scale; p.scale[1] = c->v_scale;
     p.start = start; p.count = count;
-    p.H = c->H; p.T = T; p.D = c->D; p.cap = c->capacity; p.err = ctx->dev_err;
+    p.H = c->H; p.T = T; p.D = c->D; p.cap = c->capacity; p.told = ctx->dev_err + 1;
     DEERS_CUDA_TRY(ctx, cudaSetDevice(ctx->device));
     const auto go = dtype == DEERS_F16 ? (vec ? append_launch<__half, true> : append_launch<__half, false>)
                                        : (vec ? append_launch<float, true> : append_launch<float, false>);

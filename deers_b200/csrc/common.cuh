@@ -38,8 +38,9 @@ struct deers_ctx {
     cudaStream_t stream;
     bool owns_stream;
     int sm_count;
-    // Error word the kernels write when a bounded wait gives up: dev_err in device
-    // memory, host_err its pinned host mirror, refreshed by deers_b200_sync().
+    // Error words: dev_err[0], written when a bounded wait gives up, makes the kernels behind it leave at once (their inputs may not be there);
+    // dev_err[1] tells of places and lengths outside of a cache, whose call has done its work all the same, and keeps nobody from theirs.
+    // In device memory; host_err is their pinned host mirror, refreshed by deers_b200_sync().
     unsigned int* host_err;
     unsigned int* dev_err;
     uint64_t launches;

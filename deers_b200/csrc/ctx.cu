@@ -67,18 +67,18 @@ extern "C" int deers_b200_init(int device_ordinal, void* stream, deers_ctx** out
         }
         ctx->owns_stream = true;
     }
-    // The error word lives in device memory (every CTA reads it once at start-up; a
+    // The error words live in device memory (every CTA reads the first once at start-up; a
     // host-mapped word would cost each of them a PCIe round trip) with a pinned host
     // mirror that sync() refreshes.
-    if (cudaHostAlloc((void**)&ctx->host_err, sizeof(unsigned int), cudaHostAllocDefault) != cudaSuccess ||
-        cudaMalloc((void**)&ctx->dev_err, sizeof(unsigned int)) != cudaSuccess ||
-        cudaMemset(ctx->dev_err, 0, sizeof(unsigned int)) != cudaSuccess) {
+    if (cudaHostAlloc((void**)&ctx->host_err, 2 * sizeof(unsigned int), cudaHostAllocDefault) != cudaSuccess ||
+        cudaMalloc((void**)&ctx->dev_err, 2 * sizeof(unsigned int)) != cudaSuccess ||
+        cudaMemset(ctx->dev_err, 0, 2 * sizeof(unsigned int)) != cudaSuccess) {
         if (ctx->owns_stream) cudaStreamDestroy(ctx->stream);
         if (ctx->host_err) cudaFreeHost(ctx->host_err);
         delete ctx;
         return DEERS_ERR_CUDA;
     }
-    *ctx->host_err = 0;
+    ctx->host_err[0] = ctx->host_err[1] = 0;
     for (int e = 0; e < DEERS_SCHED_ENTRIES; ++e) {
         deers_sched_entry* se = &ctx->sched[e];
         se->key[0] = -1;
@@ -185,13 +185,14 @@ extern "C" int deers_b200_memcpy_d2d(deers_ctx* ctx, void* dst, const void* src,
 
 extern "C" int deers_b200_sync(deers_ctx* ctx) {
     if (!ctx) return DEERS_ERR_NULL;
-    DEERS_CUDA_TRY(ctx, cudaMemcpyAsync(ctx->host_err, ctx->dev_err, sizeof(unsigned int), cudaMemcpyDeviceToHost,
+    DEERS_CUDA_TRY(ctx, cudaMemcpyAsync(ctx->host_err, ctx->dev_err, 2 * sizeof(unsigned int), cudaMemcpyDeviceToHost,
                                         ctx->stream));
     DEERS_CUDA_TRY(ctx, cudaStreamSynchronize(ctx->stream));
-    const unsigned int e = *(volatile unsigned int*)ctx->host_err;
+    volatile unsigned int* const words = ctx->host_err;
+    const unsigned int e = words[0] != 0 ? words[0] : words[1];
     if (e != 0) {
-        *(volatile unsigned int*)ctx->host_err = 0;
-        DEERS_CUDA_TRY(ctx, cudaMemsetAsync(ctx->dev_err, 0, sizeof(unsigned int), ctx->stream));
+        words[0] = words[1] = 0;
+        DEERS_CUDA_TRY(ctx, cudaMemsetAsync(ctx->dev_err, 0, 2 * sizeof(unsigned int), ctx->stream));
         snprintf(ctx->last_error, sizeof(ctx->last_error),
                  "kernel error word 0x%x (kernel family 0x%x, wait id %u)", e, e & 0xf00u, e & 0xffu);
         return DEERS_ERR_KERNEL;

@@ -484,7 +484,7 @@ int deers_b200_gemm_q8(deers_ctx* ctx, int32_t M, int32_t N, int32_t K, int32_t 
  *     scale' = max(scale if the block holds rows before start[b], max|new rows| * (1 / 448 in f32))
  * and where that is larger than scale the block's earlier rows are rounded again.  Nothing else changes: rows behind the last one stay as
  * they are, and appending the same rows again changes nothing.  An infinity or a NaN is stored as NaN and takes no part in the scale.  Rows outside of
- * the cache are left out and reported by the next deers_b200_sync (DEERS_ERR_KERNEL).
+ * the cache are left out and reported by the next deers_b200_sync (DEERS_ERR_KERNEL); what is enqueued behind runs all the same.
  */
 enum { DEERS_CACHE_BLOCK = 32 };
 typedef struct deers_cache_q8 {
@@ -502,7 +502,7 @@ int deers_b200_cache_q8_append(deers_ctx* ctx, const deers_cache_q8* cache, int3
  * them belong to the queries), and H query heads share the cache's heads: head h reads head h / (H / cache.H).  Query i sees keys
  * j < lengths[b] - (Tq - 1 - i) when causal, all lengths[b] otherwise; one that sees none has o = 0 and lse = -infinity.  q, o [B,H,Tq,D] f16 or
  * f32 with unit inner stride; lse [B,H,Tq] f32, may be NULL.  Sums and softmax are f32.  A length outside of [0, capacity] is taken as the nearest
- * inside and reported by the next deers_b200_sync.  Workspace: deers_b200_attn_decode_q8_workspace_bytes(desc), 0 for most calls.
+ * inside and reported by the next deers_b200_sync, what is enqueued behind runs all the same.  Workspace: deers_b200_attn_decode_q8_workspace_bytes(desc), 0 for most calls.
  */
 typedef struct deers_decode_q8_desc {
     deers_cache_q8 cache;
