@@ -12,8 +12,9 @@
 //   S^T = K Q^T: the order of the channels inside a product is free as long as K and Q agree, so a lane's 16 consecutive bytes of a key
 //   are its share of four products.  O^T += V^T P^T: the order of the keys is free too, and a lane's bytes of two keys are interleaved by
 //   byte permutations, which is the transposition that V needs.  P moves from the first product's layout to the second's by movmatrix.
-//   Weights are exp(s - m) * vs / vref * 2^15 with running maxima m (per row) and vref, as two f16 each (22 bits): the block's scale of V
-//   costs nothing per value, and small weights keep their bits.  q in f32 is two f16 as well, scaled per row by a power of two.
+//   Weights are exp(s - m) * vs * 2^K with a running maximum m, as two f16 each (22 bits): the block's scale of V costs nothing per value.  The power of two
+//   is each row's own and follows the largest exp(s - m) * vs so far, to bring it to 2^14 .. 2^15: it is products of weight and scale that keep their
+//   bits, whatever lies in blocks that a row gives no weight.  q in f32 is two f16 as well, scaled per row by a power of two.
 //   Warps meet in shared memory, the chunks of a slice in distributed shared memory (up to eight) or the workspace.
 // A row that sees no key has o = 0 and lse = -inf.  What a row does not see does not reach it, not even a NaN stored there.
 // Bound: HBM, one byte a value.
@@ -34,7 +35,7 @@ constexpr int DQ_WARPS = 4;
 constexpr int DQ_MAX_SHARES = 2 * 148, DQ_MAX_EVEN = 64;         // even shares: blocks of threads and slices at most
 constexpr int DQ_LONG = 16384;                                   // keys of a long slice
 constexpr float DQ_LOG2E = 1.4426950408889634f, DQ_LN2 = 0.6931471805599453f;
-constexpr float DQ_UP = 32768.0f;                                // weights are at most 2^15 of f16's 65504
+constexpr int DQ_UP = 15;                                        // weights are at most 2^15 of f16's 65504
 
 struct DecodeQ8Params {
     const void* q; void* o; float* lse;
@@ -69,6 +70,9 @@ __device__ __forceinline__ float power2(float x) {
     asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
     return y;
 }
+
+// 2^e, e in [-126, 127].
+__device__ __forceinline__ float power2_of(int e) { return __uint_as_float((unsigned)(127 + e) << 23); }
 
 __device__ __forceinline__ void add4(float4& v, float w, const float4& x) {
     v.x = fmaf(w, x.x, v.x); v.y = fmaf(w, x.y, v.y); v.z = fmaf(w, x.z, v.z); v.w = fmaf(w, x.w, v.w);
@@ -328,7 +332,8 @@ decode_q8_kernel(const __grid_constant__ CUtensorMap tmap_k, const __grid_consta
     }
     const int lim_min = p.causal ? len - (p.Tq - 1) : len;       // keys that every row sees
 
-    float o[NT][S::VT][4], m[NT][2], l[NT][2], vref = 0.f;
+    float o[NT][S::VT][4], m[NT][2], l[NT][2], most[NT][2];      // most: log2 of the largest weight times scale, no less than it is
+    int up[NT][2];                                               // O is held times 2^up
 #pragma unroll
     for (int nt = 0; nt < NT; ++nt) {
 #pragma unroll
@@ -337,6 +342,8 @@ decode_q8_kernel(const __grid_constant__ CUtensorMap tmap_k, const __grid_consta
             for (int e = 0; e < 4; ++e) o[nt][j][e] = 0.f;
         m[nt][0] = m[nt][1] = -INFINITY;
         l[nt][0] = l[nt][1] = 0.f;
+        most[nt][0] = most[nt][1] = -INFINITY;
+        up[nt][0] = up[nt][1] = 0;
     }
 
 #pragma unroll 1
@@ -384,16 +391,20 @@ decode_q8_kernel(const __grid_constant__ CUtensorMap tmap_k, const __grid_consta
         }
         // ---- running maxima
         const bool edge = blk * 32 + 32 > lim_min;               // (uniform)
-        const float vnew = fmaxf(vref, vs), vfac = vnew > 0.f ? vref / vnew : 0.f, vw = vnew > 0.f ? vs / vnew * DQ_UP : 0.f;
-        bool moved = vnew != vref;
-        vref = vnew;
-        float fac[NT][2];
+        // the block's scale of V is vn * 2^ve, vn in [1, 2), zero or no number
+        const bool tiny = fabsf(vs) < 1.17549435e-38f;
+        const unsigned vbits = __float_as_uint(tiny ? vs * 18446744073709551616.0f : vs);      // (times 2^64)
+        const int ve = (int)(vbits >> 23 & 0xffu) - (tiny ? 191 : 127);
+        const bool plain = vs != 0.f && ve < 128;
+        const float vn = plain ? __uint_as_float((vbits & 0x807fffffu) | 0x3f800000u) : vs, vtop = plain ? (float)(ve + 1) : -INFINITY;
+        bool moved = false;
+        float ofac[NT][2], vw[NT][2];
 #pragma unroll
         for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
             for (int x = 0; x < 2; ++x) {
                 const float f = qs[nt][x] * ks;
-                float mx = m[nt][x];
+                float here = -INFINITY;                          // the block's maximum
 #pragma unroll
                 for (int mt = 0; mt < 2; ++mt)
 #pragma unroll
@@ -408,15 +419,21 @@ decode_q8_kernel(const __grid_constant__ CUtensorMap tmap_k, const __grid_consta
 #pragma unroll
                 for (int mt = 0; mt < 2; ++mt)
 #pragma unroll
-                    for (int y = 0; y < 2; ++y) mx = fmaxf(mx, s[nt][mt][2 * y + x]);
+                    for (int y = 0; y < 2; ++y) here = fmaxf(here, s[nt][mt][2 * y + x]);
 #pragma unroll
-                for (int off = 4; off <= 16; off *= 2) mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, off));
+                for (int off = 4; off <= 16; off *= 2) here = fmaxf(here, __shfl_xor_sync(0xffffffffu, here, off));
+                const float mx = fmaxf(m[nt][x], here);
                 // (-inf: nothing seen so far, or NaN alone, which have to reach the sums)
-                const float ms = mx == -INFINITY ? 0.f : mx;
-                fac[nt][x] = power2(m[nt][x] - ms);
-                moved |= mx != m[nt][x];
+                const float ms = mx == -INFINITY ? 0.f : mx, fac = power2(m[nt][x] - ms);
                 m[nt][x] = mx;
-                l[nt][x] *= fac[nt][x];
+                l[nt][x] *= fac;
+                // Weights below 2^-110 count as 2^-110 here, which keeps vw's exponent in range.  (What fac makes zero of is no measure for the rest.)
+                most[nt][x] = fmaxf(fac > 0.f ? most[nt][x] : -INFINITY, here > -INFINITY ? fmaxf(here, ms - 110.f) + vtop : -INFINITY);
+                const int to = DQ_UP - __float2int_ru(fmaxf(most[nt][x] - ms, -300.f));
+                ofac[nt][x] = fac * power2_of(min(max(to - up[nt][x], -126), 127));
+                vw[nt][x] = vn * power2_of(min(max(to + ve, -126), 126));
+                up[nt][x] = to;
+                moved |= ofac[nt][x] != 1.f;
 #pragma unroll
                 for (int mt = 0; mt < 2; ++mt)
 #pragma unroll
@@ -432,7 +449,7 @@ decode_q8_kernel(const __grid_constant__ CUtensorMap tmap_k, const __grid_consta
 #pragma unroll
                 for (int j = 0; j < S::VT; ++j)
 #pragma unroll
-                    for (int e = 0; e < 4; ++e) o[nt][j][e] *= fac[nt][e & 1] * vfac;
+                    for (int e = 0; e < 4; ++e) o[nt][j][e] *= ofac[nt][e & 1];
         }
         // ---- weights, transposed
         uint32_t pw[NT][2][2][2];                                // [tile][16 keys][part][8 keys]
@@ -442,7 +459,7 @@ decode_q8_kernel(const __grid_constant__ CUtensorMap tmap_k, const __grid_consta
             for (int mt = 0; mt < 2; ++mt)
 #pragma unroll
                 for (int y = 0; y < 2; ++y) {
-                    const float w0 = s[nt][mt][2 * y] * vw, w1 = s[nt][mt][2 * y + 1] * vw;
+                    const float w0 = s[nt][mt][2 * y] * vw[nt][0], w1 = s[nt][mt][2 * y + 1] * vw[nt][1];
                     const uint32_t hi = pack2(w0, w1);
                     const float2 h = unpack2(hi);
                     pw[nt][mt][0][y] = transposed(hi);
@@ -471,7 +488,7 @@ decode_q8_kernel(const __grid_constant__ CUtensorMap tmap_k, const __grid_consta
 #pragma unroll
                         for (int j = 0; j < S::VT; ++j)
 #pragma unroll
-                            for (int e = 0; e < 4; ++e) o[nt][j][e] *= fac[nt][e & 1] * vfac;
+                            for (int e = 0; e < 4; ++e) o[nt][j][e] *= ofac[nt][e & 1];
                 }
 #pragma unroll
                 for (int mt = 0; mt < 2; ++mt)
@@ -485,7 +502,7 @@ decode_q8_kernel(const __grid_constant__ CUtensorMap tmap_k, const __grid_consta
                             for (int nt = 0; nt < NT; ++nt) {
                                 float w[2];
 #pragma unroll
-                                for (int x = 0; x < 2; ++x) w[x] = __shfl_sync(0xffffffffu, s[nt][mt][2 * y + x], i * 4 + t) * vw;
+                                for (int x = 0; x < 2; ++x) w[x] = __shfl_sync(0xffffffffu, s[nt][mt][2 * y + x], i * 4 + t) * vw[nt][x];
 #pragma unroll
                                 for (int j = 0; j < S::VT; ++j) {
                                     const int d = S::v_channel(j, g);
@@ -536,7 +553,7 @@ decode_q8_kernel(const __grid_constant__ CUtensorMap tmap_k, const __grid_consta
 #pragma unroll
                             for (int h = 0; h < 2; ++h) mma16816(sum, a[h][0], a[h][1], a[h][2], a[h][3], pw[nt][h][part][0], pw[nt][h][part][1]);
 #pragma unroll
-                        for (int e = 0; e < 4; ++e) to[e] = fmaf(to[e], fac[nt][e & 1] * vfac, sum[e]);
+                        for (int e = 0; e < 4; ++e) to[e] = fmaf(to[e], ofac[nt][e & 1], sum[e]);
                     } else {
 #pragma unroll
                         for (int h = 0; h < 2; ++h)
@@ -566,11 +583,18 @@ decode_q8_kernel(const __grid_constant__ CUtensorMap tmap_k, const __grid_consta
         float* mine = meet + warp * S::ROWS * S::OS;
 #pragma unroll
         for (int nt = 0; nt < NT; ++nt) {
+            float down[2][2];                                    // 2^-up in two steps: neither leaves f32 (beyond 2^-252 O is zero)
+#pragma unroll
+            for (int x = 0; x < 2; ++x) {
+                const int first = min(up[nt][x], 126);
+                down[x][0] = power2_of(-first);
+                down[x][1] = power2_of(-min(up[nt][x] - first, 126));
+            }
 #pragma unroll
             for (int j = 0; j < S::VT; ++j) {
                 const int d = S::v_channel(j, g);
 #pragma unroll
-                for (int e = 0; e < 4; ++e) mine[(nt * 8 + 2 * t + (e & 1)) * S::OS + d + (e >> 1)] = o[nt][j][e] * (1.0f / DQ_UP) * vref;      // (vref / 2^15 may be a subnormal)
+                for (int e = 0; e < 4; ++e) mine[(nt * 8 + 2 * t + (e & 1)) * S::OS + d + (e >> 1)] = o[nt][j][e] * down[e & 1][0] * down[e & 1][1];
             }
             if (g == 0) {
 #pragma unroll

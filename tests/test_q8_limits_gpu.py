@@ -5,7 +5,8 @@ import math
 import pytest
 import torch
 
-from tests.test_q8_gpu import E4M3, filled, gen, on_device, q8, same, sync
+from tests import q8_util as ref
+from tests.test_q8_gpu import TYPES, E4M3, filled, gen, near, on_device, q8, same, sync
 
 pytestmark = pytest.mark.gpu
 
@@ -86,3 +87,111 @@ def test_a_captured_step_with_a_full_sequence_serves_the_others():
     with torch.cuda.stream(side), pytest.raises(CudaError):
         ops.Context.current(torch.device("cuda", 0)).sync()
     sync()
+
+
+# ---- attention over blocks whose scales and weights are far apart ----------------------------------------------------------
+def _weighed(q, cache, lengths, scale, dtype, causal=True):
+    """(o, lse) by definition, and how far an f32 computation of o may be off: every key's share of o by the error of its own score (a sum of as many products
+    as q has channels, 2^-23 of their sizes each, and the roundings behind it), of its weight (two f16 and exp2, 2^-21) and of the sums over the keys."""
+    k, ks, v, vs = cache
+    B, H, Tq, D = q.shape
+    G, q = H // k.shape[1], q.double()
+    o, lse, err = torch.zeros_like(q), torch.full((B, H, Tq), -math.inf, dtype=torch.float64), torch.zeros_like(q)
+    for b in range(B):
+        n = int(lengths[b])
+        of = torch.arange(n) // 32
+        for h in range(H):
+            kk, vv = (t[b, h // G, :n].double() * s[b, h // G].double()[of][:, None] for t, s in ((k, ks), (v, vs)))
+            for i in range(Tq):
+                m = n - (Tq - 1 - i) if causal else n
+                if m <= 0:
+                    continue
+                s = kk[:m] @ q[b, h, i] * scale
+                p, ds = torch.softmax(s, 0), (int((q[b, h, i] != 0).sum()) + 16) * 2.0 ** -23 * (kk[:m].abs() @ q[b, h, i].abs()) * abs(scale)
+                lse[b, h, i], o[b, h, i] = torch.logsumexp(s, 0), p @ vv[:m]
+                # (the weights' sum is off by the weighed errors of the scores)
+                each = ds + float(p @ ds) + 2 * 2.0 ** -21 + 2 * (m / 8 + 64) * 2.0 ** -23
+                err[b, h, i] = (p * each) @ vv[:m].abs()
+    return o, lse, err + ref.half_step(o, dtype)
+
+
+def _far_apart(g, H, cap, D, ratio, dip, at):
+    """A cache whose keys score within a tenth of 0 along channel 0, but those of block `at`, whose scores are `dip` and whose values are `ratio` larger."""
+    k = torch.randn(1, H, cap, D, generator=g)
+    k[..., 0] = (torch.rand(1, H, cap, generator=g) - 0.5) * 0.2
+    v = torch.randn(1, H, cap, D, generator=g)
+    lo, hi = 32 * at, min(cap, 32 * at + 32)
+    k[:, :, lo:hi, 0] = dip * (1 + 0.05 * torch.rand(1, H, hi - lo, generator=g))
+    v[:, :, lo:hi] *= ratio
+    out = []
+    for t in (k, v):
+        n = -(-cap // 32)
+        p = torch.nn.functional.pad(t, (0, 0, 0, n * 32 - cap)).reshape(1, H, n, 32, D)
+        s = p.abs().amax((-1, -2)) / 448
+        out += [ref.nearest(p.double() / s.double()[..., None, None], E4M3).reshape(1, H, n * 32, D)[:, :, :cap].clone(), s]
+    return out
+
+
+# heads, query heads a head, rows, width, capacity, keys: whole slices, clusters, even shares; eight and sixteen query rows
+FAR = [(1, 1, 1, 64, 128, 100), (150, 1, 1, 64, 640, 640), (2, 1, 1, 32, 90, 90), (1, 4, 2, 128, 2048, 1500), (1, 16, 1, 96, 1000, 999), (1, 2, 1, 256, 700, 650), (1, 8, 2, 64, 16384, 3000)]
+
+
+@TYPES
+@pytest.mark.parametrize("H,G,Tq,D,cap,n", FAR, ids=lambda v: str(v))
+@pytest.mark.parametrize("ratio", [1e7, 1e9, 1e12, 1e-12], ids=lambda v: f"{v:g}")
+def test_decode_with_large_values_of_no_weight(H, G, Tq, D, cap, n, ratio, dtype):
+    """A block with values far larger than the others' and a softmax weight of e^-60: the outputs are the others', with all their bits.  In front, in the middle
+    and at the end; and values far smaller that have all the weight."""
+    g = gen(D + cap + Tq)
+    q = torch.zeros(1, H * G, Tq, D)
+    q[..., 0] = 1.0 + 0.1 * torch.rand(1, H * G, Tq, generator=g)
+    q = q.to(dtype)
+    dip = -60.0 if ratio > 1 else 60.0
+    lengths = torch.tensor([n], dtype=torch.int32)
+    for at in (0, 1, (n - 1) // 32):
+        cache = _far_apart(g, H, cap, D, ratio, dip, at)
+        got = q8().attention_decode_q8(q.cuda(), on_device(*cache), lengths.cuda(), 1.0, want_lse=True)
+        sync()
+        o, lse, err = _weighed(q, cache, lengths, 1.0, dtype)
+        near(got[0], o, err)
+
+
+@TYPES
+def test_decode_rows_weigh_large_values_each_for_itself(dtype):
+    """Of the query rows of a head some have all their weight on a block of large values and others none there; rows that do not see the block at all."""
+    g = gen(77)
+    for D, cap, n, at in ((64, 97, 97, 3), (128, 1025, 1025, 32), (64, 640, 640, 0), (128, 1025, 1025, 4)):      # (1025 and 97: the last key is a block of its own)
+        cache = _far_apart(g, 1, cap, D, 1e4, 10.0, at)
+        q = torch.zeros(1, 4, 3, D)
+        q[..., 0] = torch.tensor([1.0, -1.0, 0.0, -6.0])[None, :, None]
+        q = q.to(dtype)
+        cache[3][0, 0, at] *= 2.0 ** 30                          # values 1e13 of the others'
+        lengths = torch.tensor([n], dtype=torch.int32)
+        got = q8().attention_decode_q8(q.cuda(), on_device(*cache), lengths.cuda(), 1.0, want_lse=True)
+        sync()
+        o, lse, err = _weighed(q, cache, lengths, 1.0, torch.float32)
+        if dtype is torch.float16:                               # (values that f16 holds; the others become infinite, as they should)
+            err = err + ref.half_step(o, dtype)
+            o = torch.where(o.abs() > 65519.0, o.sign() * math.inf, o)
+        near(got[0], o, torch.where(torch.isfinite(err), err, torch.zeros_like(err)))
+
+
+def test_decode_with_values_of_every_size_beside_one_another():
+    """f32: scales from 2^-100 to 2^4 in the blocks of one walk, weights from 1 to 2^-99."""
+    g = gen(79)
+    for D, cap in ((64, 448), (128, 448)):
+        cache = _far_apart(g, 1, cap, D, 1.0, 0.0, 0)
+        n = -(-cap // 32)
+        for order in (range(n), range(n - 1, -1, -1)):
+            for i, j in enumerate(order):                        # block j: values 2^(8 i) of the smallest, scores -5.3 i (2^-7.6 i)
+                cache[3][0, 0, j] = 2.0 ** (-100 + 8 * i)
+                rows = cache[0][0, 0, 32 * j:32 * j + 32]
+                rows[:, 0] = -448.0
+                cache[1][0, 0, j] = 5.3 * i / 448 if i else 0.01 / 448
+            q = torch.zeros(1, 2, 1, D)
+            q[..., 0] = 1.0
+            lengths = torch.tensor([cap], dtype=torch.int32)
+            got = q8().attention_decode_q8(q.cuda(), on_device(*cache), lengths.cuda(), 1.0, want_lse=True)
+            sync()
+            o, lse, err = _weighed(q, cache, lengths, 1.0, torch.float32)
+            near(got[0], o, err)
