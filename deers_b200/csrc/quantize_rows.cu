@@ -7,6 +7,8 @@
 // The norm is one factor per row, so it cancels in the codes: code = nearest(h * Q / max|h|), and only the scale carries it.  One pass over
 // the row (its maximum and its sum of squares meet in one exchange), codes from the registers that hold it; the norm's rows in f32 and the
 // pass that would quantise them never exist.  Codes are the nearest to the exact quotient (q8_codes.cuh).
+// Squares of f32 values beyond 2^48 or below 2^-40 may leave f32: the sum of such a row is made again in 64 bits, from memory (in front of the codes; at the
+// kernel's end it costs every row 4 to 11 %, three sums of scaled squares as much, this 0 to 3).
 // A row of zeros has scale 0.  A row with an infinity or a NaN has scale NaN and codes 0: every product of it is NaN, as it is of the norm.
 // Bound: HBM, 7 bytes an element with f16 and a residual, 13 with f32: 16384 x 2048 f16 41 us (5.7 TB/s, 0.88 of the copy rate), 8192 x 4096 f32 79 us (0.85).
 // What it took: a row on as few threads as hold it in 40 registers, so that an SM has 1536 (48 -> 42 us; at 60 registers loads of too few rows
@@ -75,6 +77,26 @@ __device__ __forceinline__ void store_unit(T* p, int n, const T* v) {
         for (int e = 0; e < U; ++e)
             if (e < n) p[e] = v[e];
     }
+}
+
+// top / sqrt(mean(h * h) + eps) of an f32 row in 64 bits, by the tpr threads that share it; read again, which keeps the registers of the rows that do without.
+// 0 where 32 bits do, or there is nothing to divide: what squares lose above 2^-40 is less than 2^-40 of their sum, and an eps of 2^-50 outweighs those below.
+static __device__ __noinline__ float norm64(const float* x, const float* residual, int C, float top, float eps, int tid, int tpr) {
+    if (!(top > 0.f && top < __uint_as_float(0x7f800000u)) || (top < 1.f && eps >= 8.8817842e-16f)) return 0.f;
+    __shared__ double s_d[16];
+    double d = 0.0;
+    for (int at = tid; at < C; at += tpr) {
+        const double h = residual ? x[at] + residual[at] : x[at];
+        d = fma(h, h, d);
+    }
+    for (int off = 16; off >= 1; off >>= 1) d += __shfl_xor_sync(0xffffffffu, d, off);
+    if (tpr > 32) {
+        if ((tid & 31) == 0) s_d[tid >> 5] = d;
+        __syncthreads();
+        d = 0.0;
+        for (int w = 0; w < tpr / 32; ++w) d += s_d[w];
+    }
+    return (float)((double)top / sqrt(d / C + eps));
 }
 
 // TPR threads share a row (32: a warp, eight rows a block; else the block).  A thread holds NP pieces of N elements in registers, a piece being
@@ -157,9 +179,15 @@ __global__ void __launch_bounds__(TPR == 32 ? 256 : TPR, NP > 0 ? 1536 / (TPR ==
         for (int w = 0; w < W; ++w) { top = fmaxf(top, s_top[w]); ss += s_ss[w]; }
     }
     const bool number = top < __uint_as_float(0x7f800000u) && ss == ss, some = number && top > 0.f;
+    float far = 0.f;
+    if constexpr (sizeof(T) == 4 && !RELU2) {
+        // squares of values beyond 2^48, in rows of up to 2^30, may leave f32, and so may those below 2^-40 (the row's threads agree)
+        if (__builtin_expect(p.norm && !(top > 9.0949470e-13f && top < 2.8147498e14f), 0)) far = norm64(x, res, p.C, top, p.eps, tid, TPR);
+    }
     if (tid == 0) {
         float s = top;
         if (p.norm) s = top * (1.0f / sqrtf(ss * p.inv_n + p.eps));
+        if (sizeof(T) == 4 && far > 0.f) s = far;
         p.scale[row] = !number ? __uint_as_float(0x7fc00000u) : some ? s / MOST : 0.f;
     }
     const q8::Factors factors = q8::factors(MOST, top, q8::den_is_far(top));

@@ -1,12 +1,13 @@
 """The 8-bit operators where they can go wrong: places outside of a cache in front of other operators, scales of unlike sizes, rows whose squares leave
 f32, every form of the products, layouts and lengths at the ends of what is taken."""
+import ctypes
 import math
 
 import pytest
 import torch
 
 from tests import q8_util as ref
-from tests.test_q8_gpu import TYPES, E4M3, filled, gen, near, on_device, q8, same, sync
+from tests.test_q8_gpu import CODES, TYPES, E4M3, check_rows, filled, gen, near, on_device, q8, same, sync
 
 pytestmark = pytest.mark.gpu
 
@@ -195,3 +196,40 @@ def test_decode_with_values_of_every_size_beside_one_another():
             sync()
             o, lse, err = _weighed(q, cache, lengths, 1.0, torch.float32)
             near(got[0], o, err)
+
+
+# ---- the norm of rows whose squares leave f32 --------------------------------------------------------------------------------
+@CODES
+@pytest.mark.parametrize("C", [5, 64, 300, 1025, 2048, 5000, 9001, 16000])
+def test_norm_of_the_smallest_and_largest_rows(C, codes):
+    """Rows of every size of f32; the norm of one does not depend on its size (without eps)."""
+    base = torch.randn(7, C, generator=gen(C))
+    size = torch.tensor([1e36, 1e25, 3e18, 1e-18, 1e-23, 1e-30, 1e-41])
+    x = (base / base.abs().amax(1, keepdim=True) * size[:, None]).float()
+    for eps in (0.0, 1e-5):
+        h, got = q8().rms_norm_add_q8(x.cuda(), None, eps, codes)
+        sync()
+        check_rows(got, h, x, None, True, False, eps, codes)
+    x, r = (x * 0.75).float(), (x.flip(1) * 0.25).float()
+    h, got = q8().rms_norm_add_q8(x.cuda(), r.cuda(), 0.0, codes)
+    check_rows(got, h, x, r, True, False, 0.0, codes)
+
+
+@pytest.mark.parametrize("C", [40, 5000, 9001])
+def test_norm_of_the_largest_rows_into_a_callers_buffers(C):
+    """The sum in the residual's place, or in x's."""
+    from deers_b200 import _lib, ops
+    ctx = ops.Context.current(torch.device("cuda", 0))
+    x, r = (torch.randn(6, C, generator=gen(C + s)) * 1e25 for s in range(2))
+    wh, wq, ws = ref.quantize(x, r, True, False, 0.0, E4M3)
+    ld = -(-C // 16) * 16
+    for into in (0, 1):
+        dev = [x.cuda(), r.cuda()]
+        codes, scale = torch.empty(6, ld, dtype=E4M3, device="cuda"), torch.empty(6, device="cuda")
+        d = _lib.QuantizeDesc(6, C, _lib.F32, _lib.E4M3, 1, 0, 0.0, C, C, C, ld)
+        _lib.check(_lib.lib().deers_b200_quantize_rows(ctx.handle, ctypes.byref(d), dev[0].data_ptr(), dev[1].data_ptr(), dev[into].data_ptr(), codes.data_ptr(),
+                                                       scale.data_ptr()))
+        sync()
+        same(dev[into], wh)
+        same(codes[:, :C].float(), wq)
+        near(scale, ws, ws.abs() * ref.scale_tolerance(C))
