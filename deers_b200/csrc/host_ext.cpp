@@ -441,8 +441,8 @@ PyObject* gemm_q8(PyObject*, PyObject* const* args, Py_ssize_t n) {
     const int64_t K = a->size(-1), N = b->size(0);
     if (!on(b, device) || !on(sa, device) || !on(sb, device) || b->size(1) != K || K < 1 || N < 1 || !is_rows(*a) || !is_rows(*b)) Py_RETURN_NONE;
     const int64_t M = a->numel() / K;
-    if (sa->scalar_type() != at::kFloat || sb->scalar_type() != at::kFloat || !sa->is_contiguous() || !sb->is_contiguous() || sa->numel() != M || sb->numel() != N)
-        Py_RETURN_NONE;
+    if (sa->scalar_type() != at::kFloat || sb->scalar_type() != at::kFloat || !sa->is_contiguous() || !sb->is_contiguous()) Py_RETURN_NONE;
+    if (sa->sizes() != a->sizes().slice(0, a->dim() - 1) || sb->dim() != 1 || sb->size(0) != N) Py_RETURN_NONE;
     const int64_t lda = M == 1 ? (K + 15) / 16 * 16 : row_stride(*a), ldb = N == 1 ? (K + 15) / 16 * 16 : row_stride(*b);
     if (((uintptr_t)a->data_ptr() | (uintptr_t)b->data_ptr()) % 16 || (lda | ldb) % 16 || lda < K || ldb < K) Py_RETURN_NONE;
     if (M > 0x7fffffff - 512 || N > 0x7fffffff - 512 || K > 0x7fffffff - 512) Py_RETURN_NONE;

@@ -233,3 +233,18 @@ def test_norm_of_the_largest_rows_into_a_callers_buffers(C):
         same(dev[into], wh)
         same(codes[:, :C].float(), wq)
         near(scale, ws, ws.abs() * ref.scale_tolerance(C))
+
+
+# ---- products: scales of another shape ---------------------------------------------------------------------------------------
+def test_linear_refuses_scales_of_another_shape():
+    from deers_b200.errors import LayoutMismatch
+    m = q8()
+    a, w = torch.zeros(2, 3, 32, dtype=torch.int8, device="cuda"), torch.zeros(8, 32, dtype=torch.int8, device="cuda")
+    sa, sw = torch.zeros(2, 3, device="cuda"), torch.zeros(8, device="cuda")
+    assert m.linear_q8(m.RowsQ8(a, sa), m.RowsQ8(w, sw)).shape == (2, 3, 8)
+    for bad in (sa.t().contiguous(), sa.reshape(6), sa[..., None], sa[None]):
+        with pytest.raises(LayoutMismatch):
+            m.linear_q8(m.RowsQ8(a, bad), m.RowsQ8(w, sw))
+    for bad in (sw[:, None], sw[None], sw.reshape(2, 4)):
+        with pytest.raises(LayoutMismatch):
+            m.linear_q8(m.RowsQ8(a, sa), m.RowsQ8(w, bad))
