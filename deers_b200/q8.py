@@ -122,7 +122,7 @@ def linear_q8(rows: RowsQ8, weight: RowsQ8, out_dtype: torch.dtype = torch.float
     for t in (sa, b, sb):
         if t.device != a.device:
             raise DeviceMismatch(f"linear_q8: {t.device} vs {a.device}")
-    return _taken("linear_q8", _host.gemm_q8(_padded(a.reshape(-1, a.shape[-1])), sa.contiguous(), _padded(b), sb.contiguous(), out)).reshape(*a.shape[:-1], b.shape[0])
+    return _taken("linear_q8", _host.gemm_q8(_padded(a.reshape(-1, a.shape[-1])), sa.reshape(-1).contiguous(), _padded(b), sb.contiguous(), out)).reshape(*a.shape[:-1], b.shape[0])
 
 
 def _padded(codes: torch.Tensor) -> torch.Tensor:
