@@ -566,6 +566,8 @@ extern "C" int deers_b200_gemm_q8(deers_ctx* ctx, int32_t M, int32_t N, int32_t 
     if (code != DEERS_I8 && code != DEERS_E4M3) return DEERS_ERR_DTYPE;
     if (out_dtype != DEERS_F16 && out_dtype != DEERS_F32) return DEERS_ERR_DTYPE;
     if (M < 0 || N < 1 || K < 1) return DEERS_ERR_SHAPE;
+    constexpr int MOST = 0x7fffffff - 512;                       // places behind the last row or column of a tile stay within 31 bits
+    if (M > MOST || N > MOST || K > MOST) return DEERS_ERR_UNSUPPORTED;
     if (code == DEERS_I8 && K >= 131072) return DEERS_ERR_UNSUPPORTED;       // 2^31 / 128^2: sums stay whole numbers of 32 bits
     if (M == 0) return DEERS_OK;
     if (!a || !b || !c || !a_scale || !b_scale) return DEERS_ERR_NULL;

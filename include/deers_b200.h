@@ -471,7 +471,7 @@ int deers_b200_quantize_rows(deers_ctx* ctx, const deers_quantize_desc* desc, co
 /*
  * c[m, n] = a_scale[m] * b_scale[n] * sum_k a[m, k] b[n, k]: rows of codes times a weight laid out [out_features, in_features], both K
  * contiguous and of one code type.  int8 sums are exact (K < 131072); e4m3 sums are f32.  c is rounded once, to out_dtype (DEERS_F16 / DEERS_F32).
- * a, b: 16-byte aligned, lda and ldb multiples of 16; c: any leading dimension (16-byte stores where rows allow).
+ * M, N and K at most 2^31 - 513.  a, b: 16-byte aligned, lda and ldb multiples of 16; c: any leading dimension (16-byte stores where rows allow).
  */
 int deers_b200_gemm_q8(deers_ctx* ctx, int32_t M, int32_t N, int32_t K, int32_t code, const void* a, int64_t lda, const float* a_scale,
                        const void* b, int64_t ldb, const float* b_scale, int32_t out_dtype, void* c, int64_t ldc);

@@ -170,3 +170,12 @@ def test_attn_decode_q8_refuses():
         assert call(d(cache(k_strides=(ctypes.c_int64 * 3)(*strides)))) == _lib.ERR_LAYOUT
     size = lambda **c: L.deers_b200_attn_decode_q8_workspace_bytes(d(cache(**c), H=2))  # noqa: E731
     assert size(B=64, H=1, capacity=16384) > 0 and size(B=65, H=1, capacity=16384) == 0 and size(B=1, H=1, capacity=16383) == 0
+
+
+def test_gemm_q8_refuses_sizes_whose_tiles_leave_32_bits():
+    """Up to 2^31 - 513 rows, columns and summands: the last tile's places are whole numbers of 32 bits too."""
+    f = _lib.lib().deers_b200_gemm_q8
+    most = 0x7fffffff
+    for M, N, K in ((most, 8, 32), (most - 511, 8, 32), (4, most, 32), (4, most - 511, 32), (4, 8, most), (4, 8, most - 511)):
+        ld = (K + 15) // 16 * 16
+        assert f(CTX, M, N, K, _lib.E4M3, P, ld, P, P, ld, P, _lib.F16, P, N) == _lib.ERR_UNSUPPORTED, (M, N, K)
