@@ -1,9 +1,9 @@
 // Products of 8-bit rows with an 8-bit weight on tcgen05 / TMEM / TMA:
 //
-//     y[m, n] = a_scale[m] * b_scale[n] * sum_k a[m, k] b[n, k]          a [M, K], b [N, K] codes, K contiguous
+//     y[m, n] = (a_scale[m] * b_scale[n]) * sum_k a[m, k] b[n, k]          a [M, K], b [N, K] codes, K contiguous
 //
-// int8 codes (kind::i8, sums exact in 32-bit integers) or e4m3 codes (kind::f8f6f4, sums in f32); the scales and the one rounding of y are the
-// epilogue.  A K block is 128 bytes of every row, so stages, swizzle and descriptors are those of the f16 product at twice the operations a byte.
+// int8 codes (kind::i8, sums exact in 32-bit integers) or e4m3 codes (kind::f8f6f4, sums in f32, cut off); the scales and the rounding of y are the
+// epilogue.  The scales meet first: large rows and small weights bring one another back, where a sum times one of them could leave f32.  A K block is 128 bytes of every row, so stages, swizzle and descriptors are those of the f16 product at twice the operations a byte.
 // Large products go to persistent CTAs or pairs of them (8192 x 4096 x 4096 int8 89.4 us, 3070 TOP/s: 0.94 of twice the measured bf16 peak), products with few
 // tiles to clusters that share a tile's K, a step's few tokens to tiles that have the weight's rows for rows (64 x 4096 x 12288 15 us).
 // What bounds them: large ones the tensor pipe; steps the weight's bytes (here 8 us) and, before and behind them, 2 us to the first K block and 2 to 4 from the
@@ -226,7 +226,7 @@ gemm_q8_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid_constant
 #pragma unroll
                     for (int e = 0; e < PER; ++e) {
                         const int col = n0 + c0 + q * PER + e;
-                        v[e] = sum_of<I8>(r[q * PER + e]) * sa * (col < p.N ? p.sb[col] : 0.f);
+                        v[e] = sum_of<I8>(r[q * PER + e]) * (sa * (col < p.N ? p.sb[col] : 0.f));
                     }
                     pc[q] = packed<T>(v);
                 }
@@ -388,7 +388,7 @@ gemm_q8_split_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid_co
                 for (int q = 0; q < NP; ++q) {
                     float v[PER];
 #pragma unroll
-                    for (int e = 0; e < PER; ++e) v[e] = sum_of<I8>(r[q * PER + e]) * mine * scales[S::ROWS + c0 + q * PER + e];
+                    for (int e = 0; e < PER; ++e) v[e] = sum_of<I8>(r[q * PER + e]) * (mine * scales[S::ROWS + c0 + q * PER + e]);
                     pc[q] = packed<T>(v);
                 }
                 transpose_pieces<NP>(pc, (uint32_t)lane);
@@ -452,7 +452,7 @@ gemm_q8_split_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid_co
                 const float sa = scales[r0 + r];
                 float f[PER];
 #pragma unroll
-                for (int e = 0; e < PER; ++e) f[e] = sum_of<I8>(v[e]) * sa * sb[e];
+                for (int e = 0; e < PER; ++e) f[e] = sum_of<I8>(v[e]) * (sa * sb[e]);
                 if (n0 + col < p.N) store_piece<T>(p, m0 + r0 + r, n0 + col, packed<T>(f));
             }
         }

@@ -7,7 +7,7 @@ import pytest
 import torch
 
 from tests import q8_util as ref
-from tests.test_q8_gpu import CODES, TYPES, E4M3, check_rows, filled, gen, near, on_device, q8, same, sync
+from tests.test_q8_gpu import CODES, TYPES, E4M3, check_linear, check_rows, filled, gen, make_rows, near, on_device, q8, same, sync
 
 pytestmark = pytest.mark.gpu
 
@@ -248,3 +248,21 @@ def test_linear_refuses_scales_of_another_shape():
     for bad in (sw[:, None], sw[None], sw.reshape(2, 4)):
         with pytest.raises(LayoutMismatch):
             m.linear_q8(m.RowsQ8(a, sa), m.RowsQ8(w, bad))
+
+
+# ---- products: scales of every size ------------------------------------------------------------------------------------------
+@CODES
+@pytest.mark.parametrize("M,N,K", [(3, 40, 100), (300, 70, 130), (300, 70, 2400), (2500, 40, 64)], ids=lambda v: str(v))
+def test_linear_with_scales_of_every_size(M, N, K, codes):
+    """Scales whose product is in range where that of one of them and a sum is not."""
+    g = gen(M + K)
+    a, b = make_rows(g, M, K, codes)[0], make_rows(g, N, K, codes)[0]
+    for f, other in ((1e36, 1e-36), (1e-36, 1e36), (1e-42, 1e37), (1e38, 1e-30), (1e38, 1e-41)):
+        sa, sb = (((0.5 + torch.rand(n, generator=g)) * s).float() for n, s in ((M, f), (N, other)))
+        check_linear(a, sa, b, sb, codes, torch.float32)
+        if f * other <= 2:
+            check_linear(a, sa, b, sb * 2.0 ** -9, codes)
+    sa = torch.full((M,), 2.0 ** -100)
+    sa[::2] = 2.0 ** 100
+    sa[1] = 0.0
+    check_linear(a, sa, b, torch.full((N,), 2.0 ** -110), codes, torch.float32)
