@@ -490,8 +490,9 @@ GemmQ8Plan plan_gemm_q8(int sms, int pairs, int M, int N, int K) {
     for (int w = 0; w < 5; ++w) {
         const int bn = 16 << w;
         for (int swap = 0; swap < 2; ++swap) {
-            // what swapped tiles are for: as many columns as there are rows of a, 64 and 128 also several times; the others have 128 rows
-            if (swap ? (bn == 256 || bn >= 2 * M + 32 || M > (bn < 64 ? bn : 4 * bn)) : (bn < 128 || M <= 64)) continue;
+            // what swapped tiles are for: as many columns as there are rows of a, 64 also several times; the others have 128 rows (and those of 128 columns
+            // nothing over swapped ones)
+            if (swap ? (bn > 64 || bn >= 2 * M + 32 || M > (bn < 64 ? bn : 4 * bn)) : (bn < 128 || M <= 64)) continue;
             const long long tiles = swap ? up(N, QM) * up(M, bn) : up(M, QM) * up(N, bn);
             for (int ask = 1; ask <= QS_MAX_PARTS; ++ask) {
                 const int chunk = (int)up(kbs, ask), parts = (int)up(kbs, chunk);
@@ -551,7 +552,7 @@ int gemm_q8_launch(deers_ctx* ctx, const GemmQ8Params& p, const void* a, long lo
     if (rc) return rc;
     const GemmQ8Plan plan = plan_gemm_q8(ctx->sm_count, pairs, p.M, p.N, p.K);
     if (plan.split) {
-        const auto go = plan.swap ? (plan.bn == 16 ? gemm_q8_split<I8, T, 16, true> : plan.bn == 32 ? gemm_q8_split<I8, T, 32, true> : plan.bn == 64 ? gemm_q8_split<I8, T, 64, true> : gemm_q8_split<I8, T, 128, true>)
+        const auto go = plan.swap ? (plan.bn == 16 ? gemm_q8_split<I8, T, 16, true> : plan.bn == 32 ? gemm_q8_split<I8, T, 32, true> : gemm_q8_split<I8, T, 64, true>)
                                   : (plan.bn == 128 ? gemm_q8_split<I8, T, 128, false> : gemm_q8_split<I8, T, 256, false>);
         return go(ctx, p, a, lda, b, ldb, plan.parts);
     }
