@@ -41,7 +41,7 @@ SYMBOLS = [
 IPC_HANDLE_BYTES = 72
 K_FWD, K_BWD_PREP, K_BWD_MAIN, K_BWD_DQ, K_ROPE, K_OPTIM, K_NORM, K_DECODE, K_GEMM, K_GPT, K_GEMM_X3 = range(11)
 EPI_NONE, EPI_ADD, EPI_RELU_SQ, EPI_MUL_AUX2 = range(4)
-PRODUCT_F16, PRODUCT_F32, PRODUCT_F32_NORM, PRODUCT_F16X3 = range(4)
+PRODUCT_F16, PRODUCT_F32, PRODUCT_F32_NORM, PRODUCT_F16X3, PRODUCT_Q8 = range(5)
 
 
 class AttnDesc(ctypes.Structure):
@@ -99,7 +99,7 @@ class GemmEpilogue(ctypes.Structure):
 
 
 class ProductRoute(ctypes.Structure):
-    _fields_ = [(n, ctypes.c_int32) for n in ("tile_m", "tile_n", "parts", "tensor_core", "pair", "resident", "rotated")]
+    _fields_ = [(n, ctypes.c_int32) for n in ("tile_m", "tile_n", "parts", "tensor_core", "pair", "resident", "rotated", "swapped", "persistent")]
 
 
 class GptConfig(ctypes.Structure):

@@ -296,6 +296,7 @@ extern "C" int deers_b200_product_route(deers_ctx* ctx, int32_t which, int32_t n
     int rc = DEERS_OK;
     if (which == DEERS_PRODUCT_F16) rc = route_gemm_f16(ctx, M[0], N[0], K, &r);
     else if (which == DEERS_PRODUCT_F16X3) rc = route_gemm_f16x3(ctx, M[0], N[0], K, a_mn_major != 0, b_mn_major != 0, aligned, &r);
+    else if (which == DEERS_PRODUCT_Q8) rc = route_gemm_q8(ctx, M[0], N[0], K, &r);
     else if (which != DEERS_PRODUCT_F32 && which != DEERS_PRODUCT_F32_NORM) return DEERS_ERR_UNSUPPORTED;
     else if (!(rc = cluster_capacity(ctx))) {
         bool rotated = false;

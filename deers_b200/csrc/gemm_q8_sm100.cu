@@ -511,6 +511,12 @@ GemmQ8Plan plan_gemm_q8(int sms, int pairs, int M, int N, int K) {
     return best;
 }
 
+int plan_gemm_q8(deers_ctx* ctx, int M, int N, int K, GemmQ8Plan* plan, int* pairs) {
+    const int rc = gemm_f16_pairs(ctx, pairs);
+    if (!rc) *plan = plan_gemm_q8(ctx->sm_count, *pairs, M, N, K);
+    return rc;
+}
+
 template <bool I8, typename T, int BN, bool SWAP>
 int gemm_q8_split(deers_ctx* ctx, GemmQ8Params p, const void* a, long long lda, const void* b, long long ldb, int parts) {
     using S = SplitShape<BN, SWAP>;
@@ -548,9 +554,9 @@ int gemm_q8_whole(deers_ctx* ctx, const GemmQ8Params& p, const void* a, long lon
 template <bool I8, typename T>
 int gemm_q8_launch(deers_ctx* ctx, const GemmQ8Params& p, const void* a, long long lda, const void* b, long long ldb) {
     int pairs;
-    const int rc = gemm_f16_pairs(ctx, &pairs);
+    GemmQ8Plan plan;
+    const int rc = plan_gemm_q8(ctx, p.M, p.N, p.K, &plan, &pairs);
     if (rc) return rc;
-    const GemmQ8Plan plan = plan_gemm_q8(ctx->sm_count, pairs, p.M, p.N, p.K);
     if (plan.split) {
         const auto go = plan.swap ? (plan.bn == 16 ? gemm_q8_split<I8, T, 16, true> : plan.bn == 32 ? gemm_q8_split<I8, T, 32, true> : gemm_q8_split<I8, T, 64, true>)
                                   : (plan.bn == 128 ? gemm_q8_split<I8, T, 128, false> : gemm_q8_split<I8, T, 256, false>);
@@ -560,6 +566,16 @@ int gemm_q8_launch(deers_ctx* ctx, const GemmQ8Params& p, const void* a, long lo
 }
 
 }  // namespace
+
+int route_gemm_q8(deers_ctx* ctx, int M, int N, int K, deers_product_route* r) {
+    int pairs;
+    GemmQ8Plan p;
+    const int rc = plan_gemm_q8(ctx, M, N, K, &p, &pairs);
+    if (rc) return rc;
+    r->tile_m = p.swap ? p.bn : p.pair ? 2 * QM : QM; r->tile_n = p.swap ? QM : p.bn; r->parts = p.parts;
+    r->tensor_core = 1; r->pair = p.pair; r->swapped = p.swap; r->persistent = !p.split;
+    return DEERS_OK;
+}
 
 extern "C" int deers_b200_gemm_q8(deers_ctx* ctx, int32_t M, int32_t N, int32_t K, int32_t code, const void* a, int64_t lda, const float* a_scale,
                                   const void* b, int64_t ldb, const float* b_scale, int32_t out_dtype, void* c, int64_t ldc) {

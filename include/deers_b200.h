@@ -656,9 +656,10 @@ int deers_b200_selftest_umma(deers_ctx* ctx, float* max_abs_err);
  *     DEERS_PRODUCT_F32        deers_b200_gemm_f32;  aligned: rows of A and B start on 16-byte boundaries
  *     DEERS_PRODUCT_F32_NORM   the model's products of normalised rows;  heads: columns of the heads that are rotated, 0 if none are
  *     DEERS_PRODUCT_F16X3      deers_b200_gemm_f16x3 with the workspace it asks for;  aligned: rows of C do
+ *     DEERS_PRODUCT_Q8         deers_b200_gemm_q8, of either code type
  * No counterpart in the reference.
  */
-enum { DEERS_PRODUCT_F16 = 0, DEERS_PRODUCT_F32 = 1, DEERS_PRODUCT_F32_NORM = 2, DEERS_PRODUCT_F16X3 = 3 };
+enum { DEERS_PRODUCT_F16 = 0, DEERS_PRODUCT_F32 = 1, DEERS_PRODUCT_F32_NORM = 2, DEERS_PRODUCT_F16X3 = 3, DEERS_PRODUCT_Q8 = 4 };
 typedef struct deers_product_route {
     int32_t tile_m, tile_n;   /* output tile of a block, or of a pair of blocks */
     int32_t parts;            /* blocks (or passes) that share a tile's K */
@@ -666,6 +667,8 @@ typedef struct deers_product_route {
     int32_t pair;             /* two blocks work on one tile */
     int32_t resident;         /* F16X3: K blocks of A that stay in shared memory */
     int32_t rotated;          /* F32_NORM: the heads are rotated in the product's own tiles */
+    int32_t swapped;          /* Q8: the rows of the tensor core's tile are B's */
+    int32_t persistent;       /* Q8: blocks take tiles in turn, all of K each */
 } deers_product_route;
 int deers_b200_product_route(deers_ctx* ctx, int32_t which, int32_t n, const int32_t* M, const int32_t* N, int32_t K, int32_t a_mn_major,
                              int32_t b_mn_major, int32_t aligned, int32_t heads, deers_product_route* route);

@@ -7,7 +7,7 @@ import pytest
 import torch
 
 from tests import q8_util as ref
-from tests.test_q8_gpu import CODES, TYPES, E4M3, check_linear, check_rows, filled, gen, make_rows, near, on_device, q8, same, sync
+from tests.test_q8_gpu import CODES, TYPES, E4M3, I8, check_linear, check_rows, filled, gen, make_rows, near, on_device, q8, same, sync
 
 pytestmark = pytest.mark.gpu
 
@@ -266,3 +266,36 @@ def test_linear_with_scales_of_every_size(M, N, K, codes):
     sa[::2] = 2.0 ** 100
     sa[1] = 0.0
     check_linear(a, sa, b, torch.full((N,), 2.0 ** -110), codes, torch.float32)
+
+
+# ---- products: every kernel --------------------------------------------------------------------------------------------------
+# M, N, K; kernel that takes them (persistent, by pairs), columns of its tile, its rows and columns swapped, parts of K
+FORMS = [((2137, 37, 54), (True, False, 256, False, 1)), ((20001, 513, 70), (True, False, 256, False, 1)), ((5454, 1573, 609), (True, False, 256, False, 1)),
+         ((2415, 38, 3597), (True, True, 256, False, 1)), ((5423, 1541, 900), (True, True, 256, False, 1)),
+         ((138, 16196, 674), (False, False, 256, False, 1)), ((132, 6760, 6479), (False, False, 256, False, 2)), ((154, 2070, 12753), (False, False, 256, False, 7)),
+         ((513, 520, 1024), (False, False, 128, False, 1)), ((778, 777, 2879), (False, False, 128, False, 2)), ((649, 645, 2464), (False, False, 128, False, 3)),
+         ((1697, 132, 2806), (False, False, 128, False, 4)), ((333, 1001, 2731), (False, False, 128, False, 5)), ((273, 5, 2236), (False, False, 128, False, 6)),
+         ((297, 34, 2368), (False, False, 128, False, 7)), ((262, 1, 2787), (False, False, 128, False, 8)),
+         ((34, 130, 1641), (False, False, 64, True, 7)), ((35, 2395, 912), (False, False, 64, True, 4)), ((18, 3969, 1094), (False, False, 32, True, 3)),
+         ((19, 77, 916), (False, False, 32, True, 8)), ((1, 2159, 1834), (False, False, 16, True, 5))]
+
+
+@CODES
+@pytest.mark.parametrize("out", [torch.float16, torch.float32], ids=["f16", "f32"])
+@pytest.mark.parametrize("size,form", FORMS, ids=lambda v: "-".join(map(str, v)))
+def test_linear_by_every_kernel(size, form, out, codes):
+    """One size or more for every kernel, with remainders in rows, columns and K, several tiles a block, more K blocks than stages and fewer."""
+    from deers_b200 import _lib, ops
+    M, N, K = size
+    r = ops.Context.current(torch.device("cuda", 0)).product_route(_lib.PRODUCT_Q8, [(M, N)], K)
+    assert (bool(r.persistent), bool(r.pair), r.tile_m if r.swapped else r.tile_n, bool(r.swapped), r.parts) == form
+    g = gen(M + N + K)
+    a, sa = make_rows(g, M, K, codes)
+    b, sb = make_rows(g, N, K, codes, 1 / math.sqrt(K))
+    m = q8()
+    y = m.linear_q8(m.RowsQ8(a.to(codes).cuda(), sa.cuda()), m.RowsQ8(b.to(codes).cuda(), sb.cuda()), out)
+    sync()
+    a, b, both = a.cuda(), b.cuda(), (sa.double()[:, None] * sb.double()[None]).cuda()
+    want, size = (a @ b.t()) * both, (a.abs() @ b.abs().t()) * both
+    sums = 0.0 if codes is I8 else (K / 32 + 32) * 2.0 ** -23     # (as in check_linear)
+    near(y, want.cpu(), (ref.half_step(want, out) * (1 + 2.0 ** -10) + 2.0 ** -22 * want.abs() + sums * size).cpu())
