@@ -7,7 +7,7 @@ import pytest
 import torch
 
 from tests import q8_util as ref
-from tests.test_q8_gpu import CODES, TYPES, E4M3, I8, check_linear, check_rows, filled, gen, make_rows, near, on_device, q8, same, sync
+from tests.test_q8_gpu import CODES, TYPES, E4M3, I8, cache_values, check_linear, check_rows, filled, gen, make_rows, near, on_device, q8, same, sync
 
 pytestmark = pytest.mark.gpu
 
@@ -299,3 +299,43 @@ def test_linear_by_every_kernel(size, form, out, codes):
     want, size = (a @ b.t()) * both, (a.abs() @ b.abs().t()) * both
     sums = 0.0 if codes is I8 else (K / 32 + 32) * 2.0 ** -23     # (as in check_linear)
     near(y, want.cpu(), (ref.half_step(want, out) * (1 + 2.0 ** -10) + 2.0 ** -22 * want.abs() + sums * size).cpu())
+
+
+# ---- a cache with tokens in front of heads -----------------------------------------------------------------------------------
+@TYPES
+@pytest.mark.parametrize("B,H,G,Tq,D,cap", [(2, 3, 2, 1, 64, 70), (1, 5, 1, 2, 80, 300), (3, 2, 4, 4, 256, 100), (2, 1, 2, 1, 128, 90)], ids=lambda v: str(v))
+def test_a_cache_with_tokens_in_front_of_heads(B, H, G, Tq, D, cap, dtype):
+    """Codes [B, capacity, H, D] seen as [B, H, capacity, D]: append into them and attention over them."""
+    g = gen(B + H + D + cap)
+    codes = [torch.zeros(B, cap, H, D).to(E4M3).cuda().permute(0, 2, 1, 3) for _ in range(2)]
+    scales = [torch.zeros(B, H, -(-cap // 32)).cuda() for _ in range(2)]
+    c = q8().CacheQ8(codes[0], codes[1], scales[0], scales[1])
+    k, ks, v, vs = cache_values(c)
+    at = torch.zeros(B, dtype=torch.int32)
+    for T in (cap - 20, 5, Tq):
+        kn, vn = (torch.randn(B, H, T, D, generator=g).to(dtype) for _ in range(2))
+        c.append(kn.cuda(), vn.cuda(), at.cuda())
+        ref.append(k, ks, kn, at, [T] * B)
+        ref.append(v, vs, vn, at, [T] * B)
+        at += T
+    for got, want in zip(cache_values(c), (k, ks, v, vs)):
+        same(got, want)
+    q = torch.randn(B, H * G, Tq, D, generator=g).to(dtype)
+    got = q8().attention_decode_q8(q.cuda(), c, at.cuda(), want_lse=True)
+    sync()
+    o, lse, err_o, err_l = ref.decode(q, k, ks, v, vs, at, 1 / math.sqrt(D))
+    near(got[0], o, err_o[..., None] + ref.half_step(o, dtype))
+    near(got[1], lse, err_l)
+
+
+# ---- wide rows ---------------------------------------------------------------------------------------------------------------
+@CODES
+@TYPES
+@pytest.mark.parametrize("C", [8192, 12000, 16384, 16392, 20000])
+def test_wide_rows_on_16_byte_boundaries(C, dtype, codes):
+    g = gen(C)
+    x, r = torch.randn(3, C, generator=g).to(dtype), (torch.randn(3, C, generator=g) * 3).to(dtype)
+    h, got = q8().rms_norm_add_q8(x.cuda(), r.cuda(), 1e-5, codes)
+    sync()
+    check_rows(got, h, x, r, True, False, 1e-5, codes)
+    check_rows(q8().quantize_q8(x.cuda(), codes, True), None, x, None, False, True, 0.0, codes)
