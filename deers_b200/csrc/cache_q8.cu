@@ -39,7 +39,7 @@ __global__ void __launch_bounds__(128, NW == 4 && sizeof(T) == 2 ? (LR == 8 ? 10
     const int h = blockIdx.y * PER + threadIdx.x / NT, b = blockIdx.z >> 1, kv = blockIdx.z & 1;
     const bool mine = h < p.H;                                   // (with NW == 4 the whole block)
     int begin = p.start[b], n = p.count ? p.count[b] : p.T;
-    if (begin < 0 || n < 0 || n > p.T || (long long)begin + n > p.cap) {      // rows outside of the cache are left out, and told
+    if (n < 0 || n > p.T || (n > 0 && (begin < 0 || (long long)begin + n > p.cap))) {      // rows outside of the cache are left out, and told
         if (threadIdx.x == 0 && blockIdx.x == 0) atomicCAS(p.told, 0u, (unsigned)DEERS_KERR_CACHE | 1u);
         n = min(max(n, 0), p.T);
         if (begin < 0 || begin >= p.cap) n = 0;

@@ -53,6 +53,16 @@ def test_decode_of_a_length_outside_of_the_cache_leaves_other_operators_alone():
     _behind_a_report(lambda: q8().attention_decode_q8(q, c, n))
 
 
+def test_a_sequence_that_brings_no_rows_is_no_report():
+    """Idle sequences, wherever they are said to stand."""
+    c = q8().CacheQ8.new(4, 1, 10, 16)
+    new = torch.ones(4, 1, 4, 16).cuda()
+    start, count = (torch.tensor(t, dtype=torch.int32).cuda() for t in ([-1, 11, 10, 6], [0, 0, 0, 4]))
+    c.append(new, new, start, count)
+    sync()
+    assert not c.k.float()[:3].any() and not c.k_scale[:3].any() and (c.k.float()[3, 0, 6:] == 448).all()
+
+
 def test_a_captured_step_with_a_full_sequence_serves_the_others():
     """Replays of append, attention and a product where one sequence has run out of its cache: the others' rows, every time."""
     from deers_b200.errors import CudaError
