@@ -214,7 +214,7 @@ def attention_decode_q8(q, cache: CacheQ8, lengths: torch.Tensor, scale: Optiona
     [B, Hq, Tq]).  A row that sees no key has o = 0 and lse = -inf; what lies behind a sequence's last row is not read.  Of a batch padded at
     the back to T rows the lengths are ``start + T``: query t then sees rows up to its own, and what the padding's queries see is nobody's.
     Lengths beyond the capacity are taken as the capacity, and ``Context.sync`` reports them."""
-    if scale is None and q.dim() == 4:
+    if scale is None and q.dim() == 4 and q.shape[3]:
         scale = default_scale(q.shape[3])
     held = (cache.k, cache.v, cache.k_scale, cache.v_scale)
     got = _host.attn_decode_q8(*held, q, lengths, scale, causal, want_lse) if scale is not None else None

@@ -208,6 +208,14 @@ def test_decode_with_values_of_every_size_beside_one_another():
             near(got[0], o, err)
 
 
+def test_decode_refuses_queries_of_other_shapes():
+    from deers_b200.errors import LayoutMismatch
+    c, n = q8().CacheQ8.new(2, 3, 40, 32), torch.zeros(2, dtype=torch.int32, device="cuda")
+    for shape in ((2, 3, 1, 0), (2, 3, 0, 32), (2, 0, 1, 32), (1, 3, 1, 32), (2, 4, 1, 32), (2, 3, 41, 32), (2, 3, 32), (2, 3, 1, 48)):
+        with pytest.raises(LayoutMismatch):
+            q8().attention_decode_q8(torch.zeros(shape, device="cuda"), c, n)
+
+
 # ---- the norm of rows whose squares leave f32 --------------------------------------------------------------------------------
 @CODES
 @pytest.mark.parametrize("C", [5, 64, 300, 1025, 2048, 5000, 9001, 16000])
