@@ -391,12 +391,7 @@ decode_q8_kernel(const __grid_constant__ CUtensorMap tmap_k, const __grid_consta
         }
         // ---- running maxima
         const bool edge = blk * 32 + 32 > lim_min;               // (uniform)
-        // the block's scale of V is vn * 2^ve, vn in [1, 2), zero or no number
-        const bool tiny = fabsf(vs) < 1.17549435e-38f;
-        const unsigned vbits = __float_as_uint(tiny ? vs * 18446744073709551616.0f : vs);      // (times 2^64)
-        const int ve = (int)(vbits >> 23 & 0xffu) - (tiny ? 191 : 127);
-        const bool plain = vs != 0.f && ve < 128;
-        const float vn = plain ? __uint_as_float((vbits & 0x807fffffu) | 0x3f800000u) : vs, vtop = plain ? (float)(ve + 1) : -INFINITY;
+        const float vtop = (float)((int)(__float_as_uint(vs) >> 23 & 0xffu) - 126);      // vs < 2^vtop
         bool moved = false;
         float ofac[NT][2], vw[NT][2];
 #pragma unroll
@@ -427,11 +422,12 @@ decode_q8_kernel(const __grid_constant__ CUtensorMap tmap_k, const __grid_consta
                 const float ms = mx == -INFINITY ? 0.f : mx, fac = power2(m[nt][x] - ms);
                 m[nt][x] = mx;
                 l[nt][x] *= fac;
-                // Weights below 2^-110 count as 2^-110 here, which keeps vw's exponent in range.  (What fac makes zero of is no measure for the rest.)
-                most[nt][x] = fmaxf(fac > 0.f ? most[nt][x] : -INFINITY, here > -INFINITY ? fmaxf(here, ms - 110.f) + vtop : -INFINITY);
-                const int to = DQ_UP - __float2int_ru(fmaxf(most[nt][x] - ms, -300.f));
+                // Weights below 2^-110 count as 2^-110 here, so that 2^up stays in range.  (What fac makes zero of is no measure for the rest.)
+                const bool seen = here > -INFINITY;
+                most[nt][x] = fmaxf(fac > 0.f ? most[nt][x] : -INFINITY, seen ? fmaxf(here, ms - 110.f) + vtop : -INFINITY);
+                const int to = DQ_UP - __float2int_ru(fmaxf(most[nt][x] - ms, -111.f));      // -114 to 126
                 ofac[nt][x] = fac * power2_of(min(max(to - up[nt][x], -126), 127));
-                vw[nt][x] = vn * power2_of(min(max(to + ve, -126), 126));
+                vw[nt][x] = seen ? vs * power2_of(to) : 0.f;     // (a scale of any size where nothing is seen)
                 up[nt][x] = to;
                 moved |= ofac[nt][x] != 1.f;
 #pragma unroll
@@ -583,18 +579,12 @@ decode_q8_kernel(const __grid_constant__ CUtensorMap tmap_k, const __grid_consta
         float* mine = meet + warp * S::ROWS * S::OS;
 #pragma unroll
         for (int nt = 0; nt < NT; ++nt) {
-            float down[2][2];                                    // 2^-up in two steps: neither leaves f32 (beyond 2^-252 O is zero)
-#pragma unroll
-            for (int x = 0; x < 2; ++x) {
-                const int first = min(up[nt][x], 126);
-                down[x][0] = power2_of(-first);
-                down[x][1] = power2_of(-min(up[nt][x] - first, 126));
-            }
+            const float down[2] = {power2_of(-up[nt][0]), power2_of(-up[nt][1])};
 #pragma unroll
             for (int j = 0; j < S::VT; ++j) {
                 const int d = S::v_channel(j, g);
 #pragma unroll
-                for (int e = 0; e < 4; ++e) mine[(nt * 8 + 2 * t + (e & 1)) * S::OS + d + (e >> 1)] = o[nt][j][e] * down[e & 1][0] * down[e & 1][1];
+                for (int e = 0; e < 4; ++e) mine[(nt * 8 + 2 * t + (e & 1)) * S::OS + d + (e >> 1)] = o[nt][j][e] * down[e & 1];
             }
             if (g == 0) {
 #pragma unroll
