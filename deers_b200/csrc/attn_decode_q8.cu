@@ -17,7 +17,9 @@
 //   bits, whatever lies in blocks that a row gives no weight.  q in f32 is two f16 as well, scaled per row by a power of two.
 //   Warps meet in shared memory, the chunks of a slice in distributed shared memory (up to eight) or the workspace.
 // A row that sees no key has o = 0 and lse = -inf.  What a row does not see does not reach it, not even a NaN stored there.
-// Bound: HBM, one byte a value.
+// Bound: HBM, one byte a value, where slices fill the device evenly (64 x 32 heads of 2048 keys of 128, f16 161 us, 1.03 of the copy rate); with f32 queries and sixteen
+// rows instructions (two f16 parts of q and of the weights: 3 x 4 heads of 20000 to 65000 keys of 96 36 to 39 us of 15); with ragged lengths the blocks
+// that get the longest (see plan_decode_q8).
 #include <cuda_fp16.h>
 
 #include "common.cuh"
@@ -759,6 +761,10 @@ struct DecodeQ8Plan { int dp, nt, tiles, mode, splits, shares; };   // splits: b
 // again at once.  Few long slices are cut on the device in proportion to their keys, for a second launch (against 8 blocks a slice): 16 slices of
 // 65536 keys 31 / 49 us against 61 / 93, 64 of 16384 33 / 52 against 43 / 67, 16 of 16384 13 / 20 against 18 / 27.  Shorter ones gain nothing
 // (32 of 8192 keys 15 / 20 against 15 / 19; 32 of 4096 13 / 15 against 12 / 14).
+// From 65 slices on, and below 16384 keys, the cut goes by the capacity, so ragged lengths leave SMs idle: f16, D = 128, uniform from 0 / all full, of
+// the copy rate: 16 x 8 slices of 4096 keys, G 4, 25 / 31 us (0.44 / 0.67); 10 x 32 of 2048 23 / 33 (0.51 / 0.79); 16 x 32 of 2048 33 / 58 (0.57 / 0.71);
+// 40 x 8 of 4096 54 / 59 (0.51 / 0.88); 64 x 8 of 2048, G 4, 34 / 59 (0.55 / 0.71), of 8192 91 / 205 (0.76 / 0.81).
+// (148: the SMs of a B200.  The workspace's size is asked for without a context.)
 DecodeQ8Plan plan_decode_q8(const deers_decode_q8_desc* d) {
     DecodeQ8Plan p;
     p.dp = d->cache.D > 128 ? 256 : (d->cache.D + 31) / 32 * 32;

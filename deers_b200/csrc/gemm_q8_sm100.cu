@@ -4,7 +4,8 @@
 //
 // int8 codes (kind::i8, sums exact in 32-bit integers) or e4m3 codes (kind::f8f6f4, sums in f32, cut off); the scales and the rounding of y are the
 // epilogue.  The scales meet first: large rows and small weights bring one another back, where a sum times one of them could leave f32.  A K block is 128 bytes of every row, so stages, swizzle and descriptors are those of the f16 product at twice the operations a byte.
-// Large products go to persistent CTAs or pairs of them (8192 x 4096 x 4096 int8 89.4 us, 3070 TOP/s: 0.94 of twice the measured bf16 peak), products with few
+// Large products go to persistent CTAs or pairs of them (8192 x 4096 x 4096 int8 90 us, 3050 TOP/s: 0.93 of twice the measured bf16 peak, e4m3 97 to 99; without a
+// pause between calls, under the power cap, int8 104), products with few
 // tiles to clusters that share a tile's K, a step's few tokens to tiles that have the weight's rows for rows (64 x 4096 x 12288 15 us).
 // What bounds them: large ones the tensor pipe; steps the weight's bytes (here 8 us) and, before and behind them, 2 us to the first K block and 2 to 4 from the
 // last product to the end.
@@ -472,7 +473,9 @@ int tmap_bytes(deers_ctx* ctx, CUtensorMap* out, const void* base, long long row
 struct GemmQ8Plan { int bn, parts; bool swap, split, pair; };
 
 // The way with the least estimated time.  The estimate is in microseconds and was fitted to 2600 measured times (200 sizes of M 1 .. 8192, K 300 .. 16384,
-// N 512 .. 12288, every way that is meant for them); what it picks is 1.3 % slower than the best on average, 21 % at most.  Per K block a CTA needs 0.14 us with
+// N 512 .. 12288; every way that is meant for them up to M 2048, the two persistent ones above); what it picks is 1.3 % slower than the best of those on
+// average, 21 % at most.  Above M 2048 shares of K were not timed and are not picked, which leaves narrow products of long K behind: K 16384, N 512
+// take 26 us at M 2048 and 43 at 2049 and 4096; 4096 x 8192 x 256 25 (6 by its bytes).  N below 512 was not swept.  Per K block a CTA needs 0.14 us with
 // 16 columns to 0.37 with 256, a persistent one 0.45, a pair 0.33; a second CTA on an SM runs at 0.9 of the first's speed.  Adding up parts costs
 // 1.6 and 0.03 a column, a pair's launch 2.6 more than a single CTA's.  1 x 768 x 2304 6.5 us by persistent CTAs, 4.0 swapped; 64 x 4096 x 12288 19.7 and 15.0;
 // 64 x 11008 x 4096 36 and 14.3 in four parts; 333 x 2731 x 1001 29 and 10.1; 1024 x 768 x 2304 7.7 and 5.2; 8192 x 4096 x 4096 97.8, by pairs 89.4.
@@ -485,7 +488,7 @@ GemmQ8Plan plan_gemm_q8(int sms, int pairs, int M, int N, int K) {
         const double t = 6.6 + (double)up(up(M, 2 * QM) * up(N, 256), pairs) * (0.331 * kbs + 0.58);
         if (t < least) { least = t; best.pair = true; }
     }
-    if (M > 2048) return best;                                   // (never the quickest there)
+    if (M > 2048) return best;
     static const double block[5] = {0.14, 0.30, 0.28, 0.33, 0.37};
     for (int w = 0; w < 5; ++w) {
         const int bn = 16 << w;

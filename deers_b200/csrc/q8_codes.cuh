@@ -140,7 +140,7 @@ __device__ __forceinline__ uint32_t codes_of(const float (&v)[4], const Factors&
         unpack_f32x2(mul2(pack_f32x2(v[2], v[3]), pack_f32x2(f.up, f.up)), u[2], u[3]);
         constexpr float MAGIC = 12582912.0f;                      // 1.5 * 2^23: the sum's low bits are the nearest whole number
         uint32_t c[4];
-        bool near = false;                                       // (of 127 the factor is off by 2^-14.6 at most: borders are looked for 2^-13 to either side)
+        bool near = false;                                       // (of 127, 2^-22 and three roundings are 2^-14.2 at most: borders are looked for 2^-12.7 to either side)
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
             const float m = u[i] + MAGIC;

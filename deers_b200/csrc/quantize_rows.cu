@@ -10,7 +10,10 @@
 // Squares of f32 values beyond 2^48 or below 2^-40 may leave f32: the sum of such a row is made again in 64 bits, from memory (in front of the codes; at the
 // kernel's end it costs every row 4 to 11 %, three sums of scaled squares as much, this 0 to 3).
 // A row of zeros has scale 0.  A row with an infinity or a NaN has scale NaN and codes 0: every product of it is NaN, as it is of the norm.
-// Bound: HBM, 7 bytes an element with f16 and a residual, 13 with f32: 16384 x 2048 f16 41 us (5.7 TB/s, 0.88 of the copy rate), 8192 x 4096 f32 79 us (0.85).
+// Bound: HBM, 7 bytes an element with f16 and a residual, 13 with f32: 16384 x 2048 f16 42 us (int8; e4m3 41, 0.88 of the copy rate), 8192 x 4096 f32 80 (78, 0.86).
+// Rows on smaller boundaries move fewer bytes an access, codes as few at a time as values: f16 4096 x 4100 39 us (8 bytes; 0.47), 8192 x 2731 68 to 72 (2 bytes; 0.35),
+// f32 5000 x 1025 15 (4 bytes; 0.68).  Rows longer than registers hold are read twice: f32 3000 x 12000 102 to 104 (0.70), f16 2000 x 20000 68 to 70 (0.63).
+// relu^2 reads a third of the bytes and is bound by instructions: f16 16384 x 2048 28.5 us (0.55).
 // What it took: a row on as few threads as hold it in 40 registers, so that an SM has 1536 (48 -> 42 us; at 60 registers loads of too few rows
 // were in flight); borders between codes decided by exact products instead of a 64-bit division for every value next to one (relative to
 // that 51 -> 48, and new keys and values, cache_q8.cu, 141 -> 43, by remainders of f16 quotients 42.0 -> 41.3); units that neighbouring threads interleave where rows start on no 16-byte

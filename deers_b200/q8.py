@@ -12,8 +12,9 @@ loop keeps no cache.  Inference only: there are no gradients.  One block of a mo
     y = q8.linear_q8(q8.quantize_q8(o_rows), w_out)
     u = q8.quantize_q8(up, relu_squared=True)                  # between the products of the MLP
 
-Arithmetic happens in ``libdeers_b200.so``; there is no fallback.  Places and lengths live on the device, so that a captured step serves
-every length; every call allocates its outputs and workspace anew.
+Arithmetic happens in ``libdeers_b200.so``; there is no fallback.  Places and lengths live on the device, so that a captured step of these
+operators serves every length; every call allocates its outputs and workspace anew.  A rotation between projection and cache is not among them:
+``ops.RotaryPack`` takes one position for the whole batch, so sequences at unlike places are rotated by the caller.
 """
 from __future__ import annotations
 
@@ -181,8 +182,9 @@ class CacheQ8:
     def append(self, k, v, start: torch.Tensor, count: Optional[torch.Tensor] = None) -> None:
         """Row t of k and v [B, H, T, D] (f16 or f32) becomes row ``start[b] + t`` of sequence b, for t < ``count[b]`` (all T without it); start and
         count are int32 on the device.  A block of ``BLOCK`` rows keeps one scale: the largest its rows have needed since it was begun; where new
-        rows raise it, the block's earlier rows are rounded again.  Rows behind the last stay as they are.  An infinity or a NaN is kept as
-        NaN.  Rows outside of the capacity are left out, and ``Context.sync`` reports them."""
+        rows raise it, the block's earlier rows are rounded again.  Codes behind the last new row stay as they are, but not always their block's scale: a
+        sequence ends with its newest row.  An infinity or a NaN is kept as NaN.  Rows beyond the capacity, and all rows of a sequence whose
+        start is negative, are left out, and ``Context.sync`` reports them; other operators run all the same."""
         if _host.cache_append(self.k, self.v, self.k_scale, self.v_scale, k, v, start, count) is not None:
             return
         B, H, cap, D = self.k.shape
@@ -209,11 +211,12 @@ def _places(name: str, t: torch.Tensor, of: torch.Tensor) -> torch.Tensor:
 
 
 def attention_decode_q8(q, cache: CacheQ8, lengths: torch.Tensor, scale: Optional[float] = None, causal: bool = True, want_lse: bool = False):
-    """``attention_decode`` over a cache of codes: q [B, Hq, Tq, D] (f16 or f32; Hq a multiple of the cache's heads, head h reads head
+    """``attention_decode`` over a cache of codes: q [B, Hq, Tq, D] (f16 or f32; at most 128 rows; Hq a multiple of the cache's heads, head h reads head
     ``h // (Hq / H)``), ``lengths[b]`` rows of sequence b, the Tq newest of which belong to the queries.  Returns o [B, Hq, Tq, D] (and lse
     [B, Hq, Tq]).  A row that sees no key has o = 0 and lse = -inf; what lies behind a sequence's last row is not read.  Of a batch padded at
     the back to T rows the lengths are ``start + T``: query t then sees rows up to its own, and what the padding's queries see is nobody's.
-    Lengths beyond the capacity are taken as the capacity, and ``Context.sync`` reports them."""
+    The cache is read once for every 8 or 16 query rows of a head's group.  Lengths outside of the capacity are taken as the nearest inside, and
+    ``Context.sync`` reports them; other operators run all the same."""
     if scale is None and q.dim() == 4 and q.shape[3]:
         scale = default_scale(q.shape[3])
     held = (cache.k, cache.v, cache.k_scale, cache.v_scale)

@@ -112,8 +112,10 @@ int deers_b200_memcpy_d2d(deers_ctx* ctx, void* dst, const void* src, size_t byt
 
 /*
  * `Device::synchronize` (`src/device.rs:66-72` -> `src/storage/cuda.rs:1598-1602`).
- * Also reads the device error word: returns DEERS_ERR_KERNEL if any kernel since
- * the last sync gave up on a bounded wait, and clears the word.
+ * Also reads the device error words: returns DEERS_ERR_KERNEL if any kernel since
+ * the last sync gave up on a bounded wait (until then the persistent kernels behind it leave
+ * without writing their outputs) or met a token, a target, a place or a length out of range, and
+ * clears them.
  */
 int deers_b200_sync(deers_ctx* ctx);
 
@@ -484,9 +486,10 @@ int deers_b200_gemm_q8(deers_ctx* ctx, int32_t M, int32_t N, int32_t K, int32_t 
  * cache_q8_append writes row t of k and v [B,H,T,D] (f16 or f32, inner stride 1) at place start[b] + t of sequence b, for t < count[b] (T when
  * count is NULL); start and count are device arrays, so that a captured step serves every length.  Of a block that gets rows,
  *     scale' = max(scale if the block holds rows before start[b], max|new rows| * (1 / 448 in f32))
- * and where that is larger than scale the block's earlier rows are rounded again.  Nothing else changes: rows behind the last one stay as
- * they are, and appending the same rows again changes nothing.  An infinity or a NaN is stored as NaN and takes no part in the scale.  Rows outside of
- * the cache are left out and reported by the next deers_b200_sync (DEERS_ERR_KERNEL); what is enqueued behind runs all the same.
+ * and where that is larger than scale the block's earlier rows are rounded again.  Nothing else changes: codes behind the last new row stay as
+ * they are (their block's scale may not: a sequence ends with its newest row), and appending a sequence's last rows again changes nothing.  An infinity
+ * or a NaN is stored as NaN and takes no part in the scale.  Rows beyond the capacity, and all rows of a sequence whose start is negative, are left out and
+ * reported by the next deers_b200_sync (DEERS_ERR_KERNEL); what is enqueued behind runs all the same.
  */
 enum { DEERS_CACHE_BLOCK = 32 };
 typedef struct deers_cache_q8 {
@@ -503,7 +506,8 @@ int deers_b200_cache_q8_append(deers_ctx* ctx, const deers_cache_q8* cache, int3
  * Decode-time attention over such a cache: as deers_b200_attn_decode, but sequence b has lengths[b] rows (a device array; the Tq newest of
  * them belong to the queries), and H query heads share the cache's heads: head h reads head h / (H / cache.H).  Query i sees keys
  * j < lengths[b] - (Tq - 1 - i) when causal, all lengths[b] otherwise; one that sees none has o = 0 and lse = -infinity.  q, o [B,H,Tq,D] f16 or
- * f32 with unit inner stride; lse [B,H,Tq] f32, may be NULL.  Sums and softmax are f32.  A length outside of [0, capacity] is taken as the nearest
+ * f32 with unit inner stride; lse [B,H,Tq] f32, may be NULL.  Tq is at most 128 and H / cache.H * Tq at most 65535 (DEERS_ERR_UNSUPPORTED).  Sums
+ * and softmax are f32; weights (and queries in f32) enter the products as two f16 each, 22 bits.  A length outside of [0, capacity] is taken as the nearest
  * inside and reported by the next deers_b200_sync, what is enqueued behind runs all the same.  Workspace: deers_b200_attn_decode_q8_workspace_bytes(desc), 0 for most calls.
  */
 typedef struct deers_decode_q8_desc {
