@@ -3,10 +3,11 @@
 //     y[m, n] = (a_scale[m] * b_scale[n]) * sum_k a[m, k] b[n, k]          a [M, K], b [N, K] codes, K contiguous
 //
 // int8 codes (kind::i8, sums exact in 32-bit integers) or e4m3 codes (kind::f8f6f4, sums in f32, cut off); the scales and the rounding of y are the
-// epilogue.  The scales meet first: large rows and small weights bring one another back, where a sum times one of them could leave f32.  A K block is 128 bytes of every row, so stages, swizzle and descriptors are those of the f16 product at twice the operations a byte.
-// Large products go to persistent CTAs or pairs of them (8192 x 4096 x 4096 int8 90 us, 3050 TOP/s: 0.93 of twice the measured bf16 peak, e4m3 97 to 99; without a
-// pause between calls, under the power cap, int8 104), products with few
-// tiles to clusters that share a tile's K, a step's few tokens to tiles that have the weight's rows for rows (64 x 4096 x 12288 15 us).
+// epilogue.  The scales meet first: large rows and small weights bring one another back, where a sum times one of them could leave f32.
+// A K block is 128 bytes of every row, so stages, swizzle and descriptors are those of the f16 product at twice the operations a byte.
+// Large products go to persistent CTAs or pairs of them (8192 x 4096 x 4096 int8 90 us, 3050 TOP/s: 0.93 of twice the measured bf16 peak, e4m3 97 to 99;
+// without a pause between calls, under the power cap, int8 104), products with few tiles to clusters that share a tile's K, a step's few tokens to tiles
+// that have the weight's rows for rows (64 x 4096 x 12288 15 us).
 // What bounds them: large ones the tensor pipe; steps the weight's bytes (here 8 us) and, before and behind them, 2 us to the first K block and 2 to 4 from the
 // last product to the end.
 #include "sm100_ptx.cuh"
